@@ -6,6 +6,7 @@
 
 namespace mx {
 struct ConvRope;
+struct Kv8Pages;
 }
 
 extern "C" {
@@ -218,4 +219,23 @@ int mx_hs_conv_gemm(const uint16_t* x, int64_t ldx, int norm, const uint16_t* de
                     const float* gamma, float* h_out, int groups, float eps, const uint16_t* w, int64_t ldw,
                     const mx::ConvRope* a, const int32_t* pos, const int32_t* slots, uint16_t* gate, int M, int K,
                     hipStream_t stream);
+// qk_norm.hip
+int mx_qk_norm_rope(const uint16_t* qkv, int64_t ld, const uint16_t* wq, const uint16_t* wk, const float* cosb,
+                    const float* sinb, const int32_t* positions, int rows, uint16_t* q, uint16_t* k, uint16_t* v, int B,
+                    int S, int Hq, int Hkv, int D, float eps, hipStream_t stream);
+int mx_qk_norm_rope_bwd_parts(int B, int S, int Hq, int Hkv, int D);
+int mx_qk_norm_rope_bwd(const void* dq, const void* dk, const void* dv, int g32, int rep, const uint16_t* qkv, int64_t ld,
+                        const uint16_t* wq, const uint16_t* wk, const float* cosb, const float* sinb,
+                        const int32_t* positions, int rows, uint16_t* dqkv, int64_t ldo, float* part, void* dwq, void* dwk,
+                        int dw32, int B, int S, int Hq, int Hkv, int D, float eps, hipStream_t stream);
+// kv8.hip / kv8_attn.hip: the key/value cache in 8 bits (csrc/kernels/kv8_pages.h)
+int mx_kv8_append(const uint16_t* qkv, int64_t ld, const float* cosb, const float* sinb, int turns, int runs,
+                  const int32_t* index, const int32_t* slots, int n, int T, const uint16_t* wq, const uint16_t* wk,
+                  double eps, uint16_t* q, uint16_t* kout, uint16_t* vout, const mx::Kv8Pages* cache, int Hq, int D,
+                  hipStream_t stream);
+int mx_kv8_read(const mx::Kv8Pages* cache, const int32_t* slots, const int32_t* starts, const int32_t* ends, uint16_t* k,
+                uint16_t* v, int B, int n, int D, hipStream_t stream);
+int mx_kv8_attn_parts(int Hkv, int cap);
+int mx_kv8_attn(const uint16_t* q, const mx::Kv8Pages* cache, const int32_t* pos, const int32_t* slots, float* part_ml,
+                float* part_o, uint16_t* out, int B, int Hq, int D, int cap, float scale, hipStream_t stream);
 }

@@ -1,0 +1,254 @@
+// Torch op registrations of the key/value cache in 8 bits (csrc/kernels/kv8.hip, kv8_attn.hip) and of the norms of
+// query and key heads with the rotation (csrc/kernels/qk_norm.hip).
+#include "bindings_util.h"
+#include "kernels/kv8_pages.h"
+
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void check_table(const at::Tensor& cos, const at::Tensor& sin, int64_t D, const at::Tensor& like) {
+  check_f32(cos, "cos");
+  check_f32(sin, "sin");
+  MX_CHECK(cos.dim() == 2 && cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes() &&
+               cos.size(0) <= INT32_MAX && cos.device() == like.device() && sin.device() == like.device(),
+           "cos, sin: f32 [positions, D / 2] on the rows' device");
+}
+
+const int32_t* check_ints(const at::Tensor& t, at::IntArrayRef shape, const at::Tensor& like, const char* name) {
+  MX_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.sizes() == shape, name,
+           ": contiguous int32 ", shape, " on the device of the others, got ", t.scalar_type(), " ", t.sizes());
+  return t.data_ptr<int32_t>();
+}
+
+const uint16_t* check_weight(const OptTensor& w, int64_t D, const at::Tensor& like, const char* name) {
+  if (!given(w)) return nullptr;
+  check_bf16(*w, name);
+  MX_CHECK(w->dim() == 1 && w->size(0) == D && w->device() == like.device(), name, ": bf16 [", D, "] on the rows' device");
+  return bf(*w);
+}
+
+void check_heads(int64_t Hq, int64_t Hkv, int64_t D) {
+  MX_CHECK(D == 32 || D == 64 || D == 128, "heads of 32, 64 or 128 channels, got ", D);
+  MX_CHECK(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= 4096, "query heads in whole groups of a key head, got ", Hq, " of ", Hkv);
+}
+
+int64_t check_qkv(const at::Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D) {
+  const int64_t ld = check_rows_bf16(qkv, "qkv");
+  MX_CHECK(qkv.size(1) == (Hq + 2 * Hkv) * D, "qkv [T, (Hq + 2 Hkv) D], got ", qkv.sizes());
+  MX_CHECK(reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0, "qkv: rows start at multiples of 16 bytes");
+  return ld;
+}
+
+// ---------------------------------------------------------------- norms of query and key heads, rotated
+// q [B, Hq, S, D], k, v [B, Hkv, S, D] of qkv rows [B * S, (Hq + 2 Hkv) D]
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk,
+                                                            const at::Tensor& cos, const at::Tensor& sin, int64_t B,
+                                                            int64_t S, int64_t Hq, int64_t Hkv, int64_t D, double eps,
+                                                            const OptTensor& positions) {
+  check_heads(Hq, Hkv, D);
+  const int64_t ld = check_qkv(qkv, Hq, Hkv, D);
+  MX_CHECK(B >= 0 && S >= 0 && qkv.size(0) == B * S, "qkv has ", qkv.size(0), " rows, B * S = ", B * S);
+  check_table(cos, sin, D, qkv);
+  MX_CHECK(given(positions) || cos.size(0) >= S, "the table has ", cos.size(0), " positions, rows up to ", S);
+  DevGuard g(qkv.device());
+  auto q = at::empty({B, Hq, S, D}, qkv.options()), k = at::empty({B, Hkv, S, D}, qkv.options()), v = at::empty_like(k);
+  const int rc = mx_qk_norm_rope(bf(qkv), ld, check_weight(wq, D, qkv, "q_norm"), check_weight(wk, D, qkv, "k_norm"),
+                                 cos.data_ptr<float>(), sin.data_ptr<float>(),
+                                 given(positions) ? check_ints(*positions, {B * S}, qkv, "positions") : nullptr,
+                                 (int)cos.size(0), bfm(q), bfm(k), bfm(v), (int)B, (int)S, (int)Hq, (int)Hkv, (int)D,
+                                 (float)eps, cur_stream());
+  MX_CHECK(rc != -1, "qk_norm_rope: too many rows");
+  MX_OK(rc);
+  return {q, k, v};
+}
+
+// gradients [B, H, S, D] of q, k, v, all bf16 or all f32; those of k and v as whole numbers of summands a head
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk,
+                                                                const at::Tensor& dv, const at::Tensor& qkv,
+                                                                const at::Tensor& wq, const at::Tensor& wk,
+                                                                const at::Tensor& cos, const at::Tensor& sin, int64_t Hkv,
+                                                                double eps, const OptTensor& positions, int64_t out_pad,
+                                                                bool need_dw, bool dw32) {
+  MX_CHECK(dq.dim() == 4 && dk.dim() == 4 && dv.sizes() == dk.sizes(), "gradients [B, H, S, D]");
+  const int64_t B = dq.size(0), Hq = dq.size(1), S = dq.size(2), D = dq.size(3);
+  check_heads(Hq, Hkv, D);
+  const int64_t ld = check_qkv(qkv, Hq, Hkv, D);
+  const bool g32 = dq.scalar_type() == at::kFloat;
+  for (const at::Tensor& t : {dq, dk, dv}) {
+    if (g32) check_f32(t, "gradients of q, k, v");
+    else check_bf16(t, "gradients of q, k, v");
+    MX_CHECK(t.device() == qkv.device(), "gradients on the rows' device");
+  }
+  MX_CHECK(dk.size(0) == B && dk.size(2) == S && dk.size(3) == D && dk.size(1) >= Hkv && dk.size(1) % Hkv == 0 &&
+               qkv.size(0) == B * S && (g32 || dk.size(1) == Hkv),
+           "gradients of k, v [B, n Hkv, S, D] (bf16: n = 1) beside rows [B S, ..]");
+  MX_CHECK(out_pad >= 0 && out_pad % 8 == 0, "out_pad must be a non-negative multiple of 8");
+  check_table(cos, sin, D, qkv);
+  MX_CHECK(given(positions) || cos.size(0) >= S, "the table has ", cos.size(0), " positions, rows up to ", S);
+  DevGuard g(qkv.device());
+  const uint16_t *pq = check_weight(wq, D, qkv, "q_norm"), *pk = check_weight(wk, D, qkv, "k_norm");
+  const int64_t NHD = (Hq + 2 * Hkv) * D;
+  auto dqkv = empty_rows(B * S, NHD, out_pad, qkv.options());
+  const auto wo = qkv.options().dtype(dw32 ? at::kFloat : at::kBFloat16);
+  const int64_t W = need_dw ? D : 0;
+  auto dwq = B * S ? at::empty({W}, wo) : at::zeros({W}, wo), dwk = B * S ? at::empty({W}, wo) : at::zeros({W}, wo);
+  MX_CHECK(B * S <= INT32_MAX, "qk_norm_rope_bwd: too many rows");
+  auto part = at::empty({mx_qk_norm_rope_bwd_parts((int)B, (int)S, (int)Hq, (int)Hkv, (int)D), D},
+                        qkv.options().dtype(at::kFloat));
+  const int rc = mx_qk_norm_rope_bwd(dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), g32 ? 1 : 0, (int)(dk.size(1) / Hkv), bf(qkv),
+                                     ld, pq, pk, cos.data_ptr<float>(), sin.data_ptr<float>(),
+                                     given(positions) ? check_ints(*positions, {B * S}, qkv, "positions") : nullptr,
+                                     (int)cos.size(0), bfm(dqkv), NHD + out_pad, part.data_ptr<float>(),
+                                     need_dw ? dwq.data_ptr() : nullptr, need_dw ? dwk.data_ptr() : nullptr, dw32 ? 1 : 0,
+                                     (int)B, (int)S, (int)Hq, (int)Hkv, (int)D, (float)eps, cur_stream());
+  MX_CHECK(rc != -1, "qk_norm_rope_bwd: too many rows");
+  MX_OK(rc);
+  return {dqkv, dwq, dwk};
+}
+
+// ---------------------------------------------------------------- the cache in 8 bits
+// k, v uint8 [pages, Hkv, block, D], ke, ve uint8 [pages, Hkv, block / 16], table int32 [slots, max_pages]
+mx::Kv8Pages check_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ke, const at::Tensor& ve,
+                         const at::Tensor& table, const at::Tensor& like) {
+  for (const at::Tensor& t : {k, v, ke, ve}) {
+    MX_CHECK(t.device() == like.device() && t.scalar_type() == at::kByte && t.is_contiguous(),
+             "8-bit cache: contiguous uint8 tensors on the device of the rows");
+  }
+  MX_CHECK(k.dim() == 4 && k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 16 && k.size(2) % 16 == 0 &&
+               v.sizes() == k.sizes(),
+           "8-bit cache: codes [pages, Hkv, block, D] with blocks of a multiple of 16 positions, got ", k.sizes(), " and ",
+           v.sizes());
+  MX_CHECK(ke.sizes() == at::IntArrayRef({k.size(0), k.size(1), k.size(2) / 16}) && ve.sizes() == ke.sizes(),
+           "8-bit cache: exponents [pages, Hkv, block / 16], got ", ke.sizes(), " and ", ve.sizes());
+  MX_CHECK(k.numel() / k.size(3) / 16 <= INT32_MAX, "8-bit cache: too many pages");
+  for (const at::Tensor& t : {k, v}) MX_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "8-bit cache: alignment");
+  MX_CHECK(table.device() == like.device() && table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous() &&
+               table.size(0) >= 1 && table.size(1) >= 1 && table.size(0) <= INT32_MAX &&
+               table.size(1) * k.size(2) <= INT32_MAX,
+           "block table: contiguous int32 [slots, max_pages]");
+  const auto at8 = [](const at::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); };
+  return {at8(k), at8(v), at8(ke), at8(ve), table.data_ptr<int32_t>(), (int)table.size(0), (int)table.size(1),
+          (int)k.size(2), (int)k.size(0), (int)k.size(1)};
+}
+
+struct Appended {
+  at::Tensor q, k, v;
+};
+Appended append(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& index,
+                const OptTensor& slots, bool runs, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
+                const at::Tensor& ve, const at::Tensor& table, int64_t Hq, const OptTensor& wq, const OptTensor& wk,
+                double eps) {
+  const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, qkv);
+  const int64_t Hkv = kc.size(1), D = kc.size(3), T = qkv.size(0);
+  check_heads(Hq, Hkv, D);
+  const int64_t ld = check_qkv(qkv, Hq, Hkv, D);
+  check_table(cos, sin, D, qkv);
+  MX_CHECK(given(wq) == given(wk), "weights of both norms, or of none");
+  MX_CHECK(T <= INT32_MAX, "too many rows");
+  const int64_t n = runs ? index.size(0) : T;
+  const int32_t* ix = runs ? check_ints(index, {n, 4}, qkv, "runs") : check_ints(index, {T}, qkv, "pos");
+  const int32_t* sl = given(slots) ? check_ints(*slots, {T}, qkv, "slots") : nullptr;
+  DevGuard g(qkv.device());
+  Appended out;
+  if (runs) {
+    out.q = at::empty({Hq, T, D}, qkv.options());
+    out.k = at::empty({Hkv, T, D}, qkv.options());
+    out.v = at::empty_like(out.k);
+  } else {
+    out.q = at::empty({T, Hq, D}, qkv.options());
+  }
+  const int rc = mx_kv8_append(bf(qkv), ld, cos.data_ptr<float>(), sin.data_ptr<float>(), (int)cos.size(0), runs ? 1 : 0, ix,
+                               sl, (int)n, (int)T, check_weight(wq, D, qkv, "q_norm"), check_weight(wk, D, qkv, "k_norm"),
+                               eps, bfm(out.q), runs ? bfm(out.k) : nullptr, runs ? bfm(out.v) : nullptr, &pg,
+                               (int)Hq, (int)D, cur_stream());
+  MX_CHECK(rc != -1, "kv8_append: too many rows");
+  MX_OK(rc);
+  return out;
+}
+
+at::Tensor kv8_append_tokens(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
+                             const OptTensor& slots, at::Tensor kc, at::Tensor vc, at::Tensor ke, at::Tensor ve,
+                             const at::Tensor& table, int64_t Hq, const OptTensor& wq, const OptTensor& wk, double eps) {
+  return append(qkv, cos, sin, pos, slots, false, kc, vc, ke, ve, table, Hq, wq, wk, eps).q;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv8_append_prompts(const at::Tensor& qkv, const at::Tensor& cos,
+                                                                  const at::Tensor& sin, const at::Tensor& runs,
+                                                                  at::Tensor kc, at::Tensor vc, at::Tensor ke, at::Tensor ve,
+                                                                  const at::Tensor& table, int64_t Hq, const OptTensor& wq,
+                                                                  const OptTensor& wk, double eps) {
+  MX_CHECK(runs.dim() == 2 && runs.size(1) == 4, "runs int32 [n, 4] = first row, rows, slot, first position");
+  const Appended a = append(qkv, cos, sin, runs, c10::nullopt, true, kc, vc, ke, ve, table, Hq, wq, wk, eps);
+  return {a.q, a.k, a.v};
+}
+
+std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
+                                            const at::Tensor& ve, const at::Tensor& table, const OptTensor& slots,
+                                            const at::Tensor& starts, const at::Tensor& ends, int64_t n) {
+  const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, kc);
+  const int64_t Hkv = kc.size(1), D = kc.size(3);
+  check_heads(Hkv, Hkv, D);
+  MX_CHECK(starts.dim() == 1 && n >= 0 && n <= INT32_MAX, "starts int32 [B], n >= 0");
+  const int64_t B = starts.size(0);
+  const int32_t *from = check_ints(starts, {B}, kc, "starts"), *to = check_ints(ends, {B}, kc, "ends");
+  const int32_t* sl = given(slots) ? check_ints(*slots, {B}, kc, "slots") : nullptr;
+  MX_CHECK(given(slots) || B <= table.size(0), "more sequences than slots");
+  DevGuard g(kc.device());
+  auto k = at::empty({B, Hkv, n, D}, kc.options().dtype(at::kBFloat16)), v = at::empty_like(k);
+  const int rc = mx_kv8_read(&pg, sl, from, to, bfm(k), bfm(v), (int)B, (int)n, (int)D, cur_stream());
+  MX_CHECK(rc != -1, "kv8_read: too many positions");
+  MX_OK(rc);
+  return {k, v};
+}
+
+at::Tensor kv8_decode_attn(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
+                           const at::Tensor& ve, const at::Tensor& table, const at::Tensor& pos, const OptTensor& slots,
+                           int64_t max_len, double scale) {
+  check_bf16(q, "q");
+  const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, q);
+  MX_CHECK(q.dim() == 3 && q.size(2) == kc.size(3), "q [B, Hq, D], got ", q.sizes());
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = kc.size(1);
+  check_heads(Hq, Hkv, D);
+  MX_CHECK(Hq / Hkv <= 16, "up to 16 query heads a key head, got ", Hq / Hkv);
+  MX_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "q: alignment");
+  MX_CHECK(max_len >= 1, "max_len: at least one position, got ", max_len);
+  const int32_t* p = check_ints(pos, {B}, q, "pos");
+  const int32_t* sl = given(slots) ? check_ints(*slots, {B}, q, "slots") : nullptr;
+  const int64_t cap = std::min<int64_t>(max_len, (int64_t)pg.maxp * pg.block);
+  DevGuard g(q.device());
+  auto out = at::empty({B, Hq * D}, q.options());
+  const int64_t parts = mx_kv8_attn_parts((int)Hkv, (int)cap);
+  at::Tensor ml, po;
+  if (parts) {
+    ml = at::empty({B, Hq, parts, 2}, q.options().dtype(at::kFloat));
+    po = at::empty({B, Hq, parts, D}, q.options().dtype(at::kFloat));
+  }
+  const int rc = mx_kv8_attn(bf(q), &pg, p, sl, parts ? ml.data_ptr<float>() : nullptr, parts ? po.data_ptr<float>() : nullptr,
+                             bfm(out), (int)B, (int)Hq, (int)D, (int)cap, (float)scale, cur_stream());
+  MX_CHECK(rc != -1, "kv8_decode_attn: sizes not taken");
+  MX_OK(rc);
+  return out;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(mxllm, m) {
+  m.def("qk_norm_rope(Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int B, int S, int Hq, int Hkv, int D, float eps, Tensor? positions=None) -> (Tensor, Tensor, Tensor)");
+  m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor dv, Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int Hkv, float eps, Tensor? positions=None, int out_pad=0, bool need_dw=True, bool dw32=False) -> (Tensor, Tensor, Tensor)");
+  m.def("kv8_append_tokens(Tensor qkv, Tensor cos, Tensor sin, Tensor pos, Tensor? slots, Tensor(a!) k, Tensor(b!) v, Tensor(c!) ke, Tensor(d!) ve, Tensor table, int Hq, Tensor? wq, Tensor? wk, float eps) -> Tensor");
+  m.def("kv8_append_prompts(Tensor qkv, Tensor cos, Tensor sin, Tensor runs, Tensor(a!) k, Tensor(b!) v, Tensor(c!) ke, Tensor(d!) ve, Tensor table, int Hq, Tensor? wq, Tensor? wk, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("kv8_read(Tensor k, Tensor v, Tensor ke, Tensor ve, Tensor table, Tensor? slots, Tensor starts, Tensor ends, int n) -> (Tensor, Tensor)");
+  m.def("kv8_decode_attn(Tensor q, Tensor k, Tensor v, Tensor ke, Tensor ve, Tensor table, Tensor pos, Tensor? slots, int max_len, float scale) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(mxllm, CUDA, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.impl("kv8_append_tokens", &kv8_append_tokens);
+  m.impl("kv8_append_prompts", &kv8_append_prompts);
+  m.impl("kv8_read", &kv8_read);
+  m.impl("kv8_decode_attn", &kv8_decode_attn);
+}

@@ -21,8 +21,11 @@ import os
 
 import torch
 
+from torch.autograd.function import once_differentiable
+
 from . import reference as ref
-from ._ext import native, use_native
+from ..parallel.grad_ready import accum_grad
+from ._ext import native, rows_view, use_native
 
 
 def split_heads_ref(qkv: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, D: int):
@@ -129,11 +132,88 @@ def dq_mode() -> int:
     return m
 
 
+def _norm_grads(ctx, dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad):
+    """(d(qkv), dw_q, dw_k for autograd) of ``qk_norm_rope``: a weight with an owner that keeps its gradient (a trainer)
+    takes it from the f32 sums with one rounding, None for autograd then."""
+    need = ctx.needs_input_grad[1:3]
+    owned = [n and any(hasattr(w, a) for a in ("_mx_grad32", "_mx_grad_fresh", "_mx_on_grad_ready"))
+             for n, w in zip(need, ctx.leaves)]
+    dqkv, *dws = native().qk_norm_rope_bwd(dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad, any(need),
+                                           any(owned))
+    out = [None, None]
+    for i, (leaf, dw) in enumerate(zip(ctx.leaves, dws)):
+        if need[i] and not (owned[i] and accum_grad(leaf, dw)):
+            out[i] = dw.to(wq.dtype)
+    return dqkv, *out
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions):
+        q, k, v = native().qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+        ctx.save_for_backward(qkv, wq, wk, cos, sin, positions)
+        ctx.leaves = tuple(w if w.is_leaf else None for w in (wq, wk))
+        ctx.dims = (Hkv, eps)
+        return q, k, v
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv):
+        qkv, wq, wk, cos, sin, positions = ctx.saved_tensors
+        grads = _norm_grads(ctx, dq.contiguous(), dk.contiguous(), dv.contiguous(), qkv, wq, wk, cos, sin, *ctx.dims,
+                            positions, 0)
+        return *grads, None, None, None, None, None, None, None, None, None
+
+
+class _NormAttnBlockFn(torch.autograd.Function):
+    """``_AttnBlockFn`` with normed query and key heads: the backward's f32 dQ and dK / dV partials go straight into the
+    norm's backward."""
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad):
+        ops = native()
+        q, k, v = ops.qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps)
+        o, lse = ops.attn_fwd(q, k, v, causal, 1.0 / math.sqrt(D), out_pad)
+        ctx.save_for_backward(qkv, wq, wk, q, k, v, o, lse, cos, sin)
+        ctx.leaves = tuple(w if w.is_leaf else None for w in (wq, wk))
+        ctx.dims = (Hkv, eps, causal, grad_pad)
+        return o.view(B * S, Hq * D)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        qkv, wq, wk, q, k, v, o, lse, cos, sin = ctx.saved_tensors
+        Hkv, eps, causal, grad_pad = ctx.dims
+        dq, dkp, dvp = attn_bwd(do.contiguous(), q, k, v, o, lse, causal, 1.0 / math.sqrt(q.shape[3]), dq_mode())
+        grads = _norm_grads(ctx, dq, dkp, dvp, qkv, wq, wk, cos, sin, Hkv, eps, None, grad_pad)
+        return *grads, None, None, None, None, None, None, None, None, None, None, None
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 B: int, S: int, Hq: int, Hkv: int, D: int, eps: float = 1e-5, positions: torch.Tensor | None = None):
+    """RMS norm of every query and key head (weights ``q_norm``, ``k_norm`` [D]) and its rotation, in one pass:
+    qkv [B * S, (Hq + 2 Hkv) D] -> q [B, Hq, S, D], k and v [B, Hkv, S, D] as the attention kernels take them.
+    A row's position is its place in its sequence, or ``positions`` [B * S] int32 (packed documents); what lies outside
+    the table ``cos``, ``sin`` [positions, D / 2] comes out as NaN.  Differentiable once, in qkv and both weights
+    (csrc/kernels/qk_norm.hip)."""
+    if use_native(qkv):
+        return _QKNormRopeFn.apply(rows_view(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+    return ref.qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+
+
 def attention_block(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, B: int, S: int, Hq: int,
-                    Hkv: int, D: int, causal: bool = True, out_pad: int = 0, grad_pad: int = 0) -> torch.Tensor:
+                    Hkv: int, D: int, causal: bool = True, out_pad: int = 0, grad_pad: int = 0,
+                    norms: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
     """qkv [B*S, (Hq+2Hkv)*D] -> attention output [B*S, Hq*D] (RoPE at positions 0..S-1).
     ``out_pad`` / ``grad_pad``: padded row layouts of the output and of d(qkv)
-    for LoRA-augmented GEMM neighbours (mxllm/ops/linear.py)."""
+    for LoRA-augmented GEMM neighbours (mxllm/ops/linear.py).
+    ``norms`` (q_norm [D], k_norm [D], eps): the heads are normed before they are rotated (``qk_norm_rope``)."""
+    if norms is not None:
+        wq, wk, eps = norms
+        if use_native(qkv):
+            return _NormAttnBlockFn.apply(rows_view(qkv), wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad)
+        q, k, v = ref.qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps)
+        return ref.attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal=causal).reshape(B * S, Hq * D)
     if use_native(qkv):
         return _AttnBlockFn.apply(qkv.contiguous(), cos, sin, B, S, Hq, Hkv, D, causal, out_pad, grad_pad)
     q, k, v = split_heads_ref(qkv, B, S, Hq, Hkv, D)

@@ -55,6 +55,23 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).to(x.dtype)
 
 
+def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 B: int, S: int, Hq: int, Hkv: int, D: int, eps: float, positions: torch.Tensor | None = None):
+    """qkv rows [B * S, (Hq + 2 Hkv) D] -> q [B, Hq, S, D], k, v [B, Hkv, S, D]: every query and key head RMS-normed, then
+    rotated at its row's position; f32 in between, one rounding."""
+    x = qkv.view(B, S, Hq + 2 * Hkv, D)
+    pos = torch.arange(S, device=qkv.device).expand(B, S) if positions is None else positions.view(B, S).long()
+    c, s = cos[pos][:, :, None].float(), sin[pos][:, :, None].float()
+
+    def one(h, w):
+        h = h.float()
+        h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        a, b = h[..., :D // 2], h[..., D // 2:]
+        return torch.cat([a * c - b * s, b * c + a * s], -1).to(qkv.dtype).transpose(1, 2).contiguous()
+
+    return one(x[:, :, :Hq], q_norm), one(x[:, :, Hq:Hq + Hkv], k_norm), x[:, :, Hq + Hkv:].transpose(1, 2).contiguous()
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
               scale: float | None = None) -> torch.Tensor:
     """q [B, S, Hq, D], k/v [B, Sk, Hkv, D] -> o [B, S, Hq, D]  (GQA, fp32 math).
