@@ -235,7 +235,7 @@ int mx_kv8_append(const uint16_t* qkv, int64_t ld, const float* cosb, const floa
                   hipStream_t stream);
 int mx_kv8_read(const mx::Kv8Pages* cache, const int32_t* slots, const int32_t* starts, const int32_t* ends, uint16_t* k,
                 uint16_t* v, int B, int n, int D, hipStream_t stream);
-int mx_kv8_attn_parts(int Hkv, int cap);
+int mx_kv8_attn_parts(int B, int Hkv, int D, int cap);
 int mx_kv8_attn(const uint16_t* q, const mx::Kv8Pages* cache, const int32_t* pos, const int32_t* slots, float* part_ml,
                 float* part_o, uint16_t* out, int B, int Hq, int D, int cap, float scale, hipStream_t stream);
 }

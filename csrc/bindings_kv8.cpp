@@ -215,12 +215,13 @@ at::Tensor kv8_decode_attn(const at::Tensor& q, const at::Tensor& kc, const at::
   MX_CHECK(Hq / Hkv <= 16, "up to 16 query heads a key head, got ", Hq / Hkv);
   MX_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "q: alignment");
   MX_CHECK(max_len >= 1, "max_len: at least one position, got ", max_len);
+  MX_CHECK(scale > 0 && scale <= 3.4028234663852886e38, "scale: a positive number, got ", scale);
   const int32_t* p = check_ints(pos, {B}, q, "pos");
   const int32_t* sl = given(slots) ? check_ints(*slots, {B}, q, "slots") : nullptr;
   const int64_t cap = std::min<int64_t>(max_len, (int64_t)pg.maxp * pg.block);
   DevGuard g(q.device());
   auto out = at::empty({B, Hq * D}, q.options());
-  const int64_t parts = mx_kv8_attn_parts((int)Hkv, (int)cap);
+  const int64_t parts = mx_kv8_attn_parts((int)B, (int)Hkv, (int)D, (int)cap);
   at::Tensor ml, po;
   if (parts) {
     ml = at::empty({B, Hq, parts, 2}, q.options().dtype(at::kFloat));

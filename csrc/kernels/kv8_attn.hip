@@ -1,37 +1,44 @@
 // Attention of one token of each sequence over a paged cache of 8 bits (kv8.h):
 //   o = softmax(q k^T scale) v over positions 0 .. pos, queries of a group of heads sharing a key/value head.
 //
-// Bound by memory: a key and a value of a head are 2 D bytes and half of a bf16 cache's, each read once for all query heads of
-// the group.  Codes become bf16 in registers, where they are exact; the powers of two of a unit (16 positions) go
-// into its scores and its weights, so they cost a product a score and a weight:
-//   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += V^T . (2^(ev - 127) P)
-// by v_mfma_f32_16x16x32_bf16.  Maxima, sums and outputs are f32; a weight is rounded once to bf16 (2^-9 of it, in a sum of
-// many) where the product takes it, while the sum under it takes what was not rounded.
+// Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
+// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 55 us, where loads alone take 53 and a linear read of as much 45.
 //
-// The operands: a lane (c, g) of K has row c of a unit and the channels 64 (s / 2) + 16 g + 8 (s % 2) .. of step s (a dot
-// product does not mind the order, so a lane takes whole pieces of 16 bytes; Q is laid out alike), of V eight rows and D / 16
-// neighbouring channels, whose bytes are put together row by row as the product reads them.  No tile goes through LDS.
+// Scores by v_mfma_scale_f32_16x16x128_f8f6f4 on the codes themselves: keys as they lie, under their unit's (16 positions)
+// exponent byte, queries as sums of two e4m3 codes (Kv8Query).  Codes as bf16 cost 32 conversions a tile and the query's
+// products nothing less: 40 x 1000 .. 4000 keys of 64 18.1 -> 16.2 us, 64 x 30 .. 512 of 128 13.5 -> 11.1, long ones alike.
+//   S^T[key][head] = 2^(ek - 127) 2^(eq - 127) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
+// The outputs by v_mfma_f32_16x16x32_bf16: values become bf16 in registers, where they are exact, and a weight is rounded
+// once to bf16 (2^-8 of it, in a sum of many), while the sum under it takes what was not rounded.  Sums and outputs are f32.
 //
-// Keys are dealt evenly: the units of all sequences in a row are cut into equal shares, one a workgroup of a KV head, whose four
-// waves share what it has of a sequence; sequences that were cut are merged by a second launch.
+// The operands: a lane (c, g) of K has row c of a unit and the channels 64 h + 16 g .. + 15 (a dot product does not mind the
+// order, so a lane takes whole pieces of 16 bytes; queries are laid out alike), of V eight rows and D / 16 neighbouring
+// channels, whose bytes are put together row by row as the product reads them.  No tile goes through LDS.  Loads of the next
+// tile ahead of the products of the last, and more waves a CU, change nothing.
+//
+// Rows are whole (a workgroup each, nothing to merge) or cut: the units of all sequences in a row are dealt in equal
+// shares, one a workgroup of a KV head, whose four waves share what it has of a sequence, and sequences that were cut are
+// merged by a second launch.  Where a row is cut follows from the lengths of all, so the last bits of an output may
+// differ from batch to batch (the same call has the same bits).
 #include "kv8.h"
 
 namespace mx {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ f32x4 mfma16(const u16x8& a, const u16x8& b, const f32x4& c) {
+__device__ __forceinline__ f32x4 mfma16(const u32x4v& a, const u16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
 }
-__device__ __forceinline__ uint32_t pair_bf16(uint32_t w, bool high) {
-  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))
-              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+// codes a under 2^(ea - 127) (one of each row), codes b under 2^(eb - 127) (one of each column)
+__device__ __forceinline__ f32x4 mfma128(const i32x8& a, const i32x8& b, const f32x4& c, int ea, int eb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, ea, 0, eb);
 }
-// channel of k-step s of lane group g
-template <int D>
-__device__ __forceinline__ int chan(int s, int g) {
-  return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t w, float scale, bool high) {
+  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
 }
 
 template <int E>
@@ -50,10 +57,53 @@ __device__ __forceinline__ uint32_t word(uint2 v, int i) { return i ? v.y : v.x;
 __device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
 __device__ __forceinline__ uint32_t word(uint16_t v, int) { return v; }
 
+// A head's query as codes: high, the nearest e4m3 of q 2^s, and low, the nearest of what is left, s such that the largest channel
+// is in [128, 256).  A bf16 number is their sum exactly where it is at least 2^-10 of the largest channel, and off by 2^-18 of
+// that below.  Laid out as the lane (c, g) has its channels of a key: head c.
+template <int D>
+struct Kv8Query {
+  static constexpr int PARTS = D == 128 ? 2 : 1;  // products a unit: high and low in one where a head leaves room
+  i32x8 q[PARTS];
+  int e;  // its power of two
+
+  __device__ __forceinline__ void load(const uint16_t* row, bool on, int g) {
+    constexpr int N = D / 4;  // channels of a lane
+    float x[N];
+    float top = 0.f;
+#pragma unroll
+    for (int h = 0; h < N / 8; ++h) {
+      const u16x8 v = *reinterpret_cast<const u16x8*>(row + (D == 32 ? 8 * g : 64 * (h >> 1) + 16 * g + 8 * (h & 1)));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[8 * h + j] = on ? bf2f(v[j]) : 0.f;
+        top = fmaxf(top, fabsf(x[8 * h + j]));
+      }
+    }
+    top = lane_max<32>(lane_max<16>(top));
+    e = max((int)(__float_as_uint(top) >> 23), 8) - 7;  // (2^-120 and less: as codes of 2^-120)
+    uint32_t hi[N / 4], lo[N / 4];
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      hi[w] = kv8_code4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3], 127 - e);
+      float y[4];
+      kv8_value4(hi[w], e - 127, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = x[4 * w + j] - y[j];
+      lo[w] = kv8_code4(y[0], y[1], y[2], y[3], 127 - e);
+    }
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if constexpr (D == 128) q[0][w] = hi[w], q[1][w] = lo[w];
+      else if constexpr (D == 64) q[0][w] = w < 4 ? hi[w & 3] : lo[w & 3];
+      else q[0][w] = w < 2 ? hi[w & 1] : w < 4 ? lo[w & 1] : 0;
+    }
+  }
+};
+
 template <int D>
 struct Kv8State {  // of one wave
-  static constexpr int E = D / 16, KS = D / 32;
-  float m, l;   // of head c; l: this lane's keys
+  static constexpr int E = D / 16, KW = D / 16;  // channels of V and words of K that a lane has of a row
+  float m, l;   // reference of the exponents of head c; l: this lane's keys
   f32x4 o[E];   // [e][i]: channel E (4 g + i) + e of head c
 
   __device__ __forceinline__ void clear() {
@@ -62,102 +112,111 @@ struct Kv8State {  // of one wave
     for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // two units; k0, v0 / k1, v1: their rows, ks / vs: what their scores / weights are multiplied by, lim: their last row that is
-  // there (-1: none; rows behind it are read as that row, and count nothing)
-  __device__ __forceinline__ void take(const uint8_t* __restrict__ k0, const uint8_t* __restrict__ k1,
-                                       const uint8_t* __restrict__ v0, const uint8_t* __restrict__ v1, float ks0, float ks1,
-                                       float vs0, float vs1, int lim0, int lim1, const u16x8 (&qf)[KS], int c, int g) {
-    uint32_t k[2][2 * KS];  // words of the lane's channels, in the order of the k-steps
+  // two units of one wave, on their way from memory
+  struct Tile {
+    uint32_t k[2][KW];
     typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
+  };
+  // k0, v0 / k1, v1: the units; ALL: every row of both is there; else lim: their last one (less than 0: none), and rows behind it
+  // are read as that row
+  template <bool ALL>
+  static __device__ __forceinline__ void load(Tile& t, const uint8_t* __restrict__ k0, const uint8_t* __restrict__ k1,
+                                              const uint8_t* __restrict__ v0, const uint8_t* __restrict__ v1, int lim0,
+                                              int lim1, int c, int g) {
     const int z0 = max(lim0, 0), z1 = max(lim1, 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint8_t* p = (j ? k1 : k0) + (uint32_t)(min(c, j ? z1 : z0) * D);
+      const uint8_t* p = (j ? k1 : k0) + (uint32_t)((ALL ? c : min(c, j ? z1 : z0)) * D + (D == 32 ? 8 : 16) * g);
       if constexpr (D == 32) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p + 8 * g);
-        k[j][0] = w.x, k[j][1] = w.y;
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        t.k[j][0] = w.x, t.k[j][1] = w.y;
       } else {
 #pragma unroll
         for (int h = 0; h < D / 64; ++h) {
-          const uint4 w = *reinterpret_cast<const uint4*>(p + 64 * h + 16 * g);
-          k[j][4 * h] = w.x, k[j][4 * h + 1] = w.y, k[j][4 * h + 2] = w.z, k[j][4 * h + 3] = w.w;
+          const uint4 w = *reinterpret_cast<const uint4*>(p + 64 * h);
+          t.k[j][4 * h] = w.x, t.k[j][4 * h + 1] = w.y, t.k[j][4 * h + 2] = w.z, t.k[j][4 * h + 3] = w.w;
         }
       }
     }
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      v[s] = *reinterpret_cast<const typename VPiece<E>::type*>((s < 4 ? v0 : v1) +
-                                                                (uint32_t)(min(4 * g + (s & 3), s < 4 ? z0 : z1) * D + E * c));
-    __builtin_amdgcn_sched_barrier(0);  // every load is in flight before the first product waits
+    for (int s = 0; s < 8; ++s) {
+      const int r = ALL ? 4 * g + (s & 3) : min(4 * g + (s & 3), s < 4 ? z0 : z1);
+      t.v[s] = *reinterpret_cast<const typename VPiece<E>::type*>((s < 4 ? v0 : v1) + (uint32_t)(r * D + E * c));
+    }
+  }
+
+  // ke: exponent bytes of the units' keys, vs: powers of two of their values
+  template <bool ALL>
+  __device__ __forceinline__ void take(const Tile& t, const Kv8Query<D>& qf, float sl, int ke0, int ke1, float vs0, float vs1,
+                                       int lim0, int lim1, int g) {
     f32x4 sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      i32x8 a;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) sc[j] = mfma16(dequant8(k[j][2 * s], k[j][2 * s + 1]), qf[s], sc[j]);
-    }
-    float mx = m;
+      for (int w = 0; w < 8; ++w) a[w] = (int)t.k[j][w % KW];
+      const int ke = j ? ke1 : ke0;
+      sc[j] = mfma128(a, qf.q[0], f32x4{0.f, 0.f, 0.f, 0.f}, ke, qf.e);
+      if constexpr (Kv8Query<D>::PARTS > 1) sc[j] = mfma128(a, qf.q[1], sc[j], ke, qf.e);
+      if (!ALL) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = 4 * g + i <= (j ? lim1 : lim0) ? sc[j][i] * (j ? ks1 : ks0) : -INFINITY;
-        sc[j][i] = x;
-        mx = fmaxf(mx, x);
+        for (int i = 0; i < 4; ++i) sc[j][i] = 4 * g + i <= (j ? lim1 : lim0) ? sc[j][i] : -INFINITY;
       }
-    mx = lane_max<32>(lane_max<16>(mx));
-    const float mref = mx == -INFINITY ? 0.f : mx, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mref);
-    m = mx;
-    l *= f;
+    }
+    // The exponents' reference is a maximum that may be behind by 2^8: weights up to there cost no precision, and the sums are
+    // multiplied again in a few of the tiles only
+    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                      fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl;
+    if (__ballot(top > m + 8.f)) {
+      const float now = fmaxf(m, lane_max<32>(lane_max<16>(top))), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= f;
+      for (int e = 0; e < E; ++e) o[e] *= f;
+    }
+    const float mref = m == -INFINITY ? 0.f : m;
     u16x8 pb;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(sc[j][i] - mref);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], sl, -mref));
         l += p;
-        pb[4 * j + i] = f2bf(p * (j ? vs1 : vs0));
+        pb[4 * j + i] = f2bf(p);
       }
-    // bytes 0, 1 (lo) or 2, 3 (hi) of the words of two rows side by side, as pairs of rows of one channel each
+    // bytes 0, 1 or 2, 3 of the words of two rows side by side, as pairs of rows of one channel each
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-      u32x4 a0, a1;
+      u32x4v a0, a1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w = __builtin_amdgcn_perm(word(v[2 * i + 1], e >> 2), word(v[2 * i], e >> 2),
+        const uint32_t w = __builtin_amdgcn_perm(word(t.v[2 * i + 1], e >> 2), word(t.v[2 * i], e >> 2),
                                                  e & 2 ? 0x07030602u : 0x05010400u);
-        a0[i] = pair_bf16(w, false), a1[i] = pair_bf16(w, true);
+        a0[i] = pair_bf16(w, i < 2 ? vs0 : vs1, false), a1[i] = pair_bf16(w, i < 2 ? vs0 : vs1, true);
       }
-      o[e] = mfma16(__builtin_bit_cast(u16x8, a0), pb, o[e]);
-      o[e + 1] = mfma16(__builtin_bit_cast(u16x8, a1), pb, o[e + 1]);
+      o[e] = mfma16(a0, pb, o[e]);
+      o[e + 1] = mfma16(a1, pb, o[e + 1]);
     }
   }
 };
 
-// keys of row b: none where its slot is none of the table's
-__device__ __forceinline__ int kv8_len(const int32_t* pos, const int32_t* slots, const Kv8Pages& pg, int cap, int b) {
-  const int slot = slots ? slots[b] : b;
-  return (unsigned)slot < (unsigned)pg.slots ? min(max(pos[b], -1), cap - 1) + 1 : 0;
+// keys of a row: none where its slot is none of the table's
+__device__ __forceinline__ int kv8_len(int pos, int slot, const Kv8Pages& pg, int cap) {
+  return (unsigned)slot < (unsigned)pg.slots ? min(max(pos, -1), cap - 1) + 1 : 0;
 }
-// units that row b is dealt as: its own and kPad for what a workgroup spends on a row beside its keys
+// units that a row of `len` keys is dealt as: its own and kPad for what a workgroup spends on a row beside its keys
 constexpr int kPad = 6, kLeast = 8;
-__device__ __forceinline__ int kv8_dealt(const int32_t* pos, const int32_t* slots, const Kv8Pages& pg, int cap, int b) {
-  const int n = (kv8_len(pos, slots, pg, cap, b) + kUnit - 1) / kUnit;
-  return n ? n + kPad : 0;
-}
+__device__ __forceinline__ int kv8_dealt(int len) { return len ? (len + kUnit - 1) / kUnit + kPad : 0; }
 __device__ __forceinline__ int kv8_share(int total, int W) { return max((total + W - 1) / W, kLeast); }
 
 // EVEN: grid (W, Hkv), shares of all rows' units; else (Hkv, B), a workgroup a row.
 template <int D, int WAVES, bool EVEN>
-__global__ void __launch_bounds__(64 * WAVES)
+__global__ void __launch_bounds__(64 * WAVES, 3)
     kv8_attn_kernel(const uint16_t* __restrict__ q, Kv8Pages pg, const int32_t* __restrict__ pos,
                     const int32_t* __restrict__ slots, float* __restrict__ part_ml, float* __restrict__ part_o,
                     uint16_t* __restrict__ out, int B, int Hq, int cap, int nparts, float sl) {
   typedef Kv8State<D> State;
-  constexpr int E = State::E, KS = State::KS, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
+  constexpr int E = State::E, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
   typedef float orow_t __attribute__((ext_vector_type(E)));
   __shared__ __attribute__((aligned(32))) float so[WAVES * 16 * ROW];
   __shared__ float mls[WAVES][2][16];
@@ -165,31 +224,41 @@ __global__ void __launch_bounds__(64 * WAVES)
   const int c = lane & 15, g = lane >> 4, rep = Hq / pg.Hkv;
   const int hk = EVEN ? blockIdx.y : blockIdx.x;
   int b = EVEN ? 0 : blockIdx.y, start = 0, at = 0, end = 0, share = 1;
+  int i0 = 0, lens = 0, at_slot = 0;  // EVEN: lane i has row i0 + i
+  const auto window = [&](int from) {
+    i0 = from;
+    at_slot = from + lane < B ? (slots ? slots[from + lane] : from + lane) : -1;
+    lens = from + lane < B ? kv8_len(pos[from + lane], at_slot, pg, cap) : 0;
+    return kv8_dealt(lens);
+  };
   if constexpr (EVEN) {
-    int total = 0;
-    for (int i = lane; i < B; i += 64) total += kv8_dealt(pos, slots, pg, cap, i);
+    int total = 0, mine = 0;
+    for (int f = 64 * ((B - 1) / 64); f >= 0; f -= 64) total += mine = window(f);  // (the first rows stay)
     total = __builtin_amdgcn_readfirstlane(wave_sum(total));
     share = kv8_share(total, gridDim.x);
     at = blockIdx.x * share;
     end = min(total, at + share);
     if (at >= end) return;
-    for (int i0 = 0;; i0 += 64) {  // the row that holds unit `at`: start <= at < start + its units
-      const int n = i0 + lane < B ? kv8_dealt(pos, slots, pg, cap, i0 + lane) : 0;
-      const int upto = (int)wave_scan((uint32_t)n);
+    while (true) {  // the row that holds unit `at`: start <= at < start + its units
+      const int upto = (int)wave_scan((uint32_t)mine);
       const uint64_t past = __ballot(start + upto > at);
       if (past) {
         const int first = __ffsll((unsigned long long)past) - 1;
         b = __builtin_amdgcn_readfirstlane(i0 + first);
-        start = __builtin_amdgcn_readlane(start + upto - n, first);
+        start = __builtin_amdgcn_readlane(start + upto - mine, first);
         break;
       }
       start = __builtin_amdgcn_readlane(start + upto, 63);
+      mine = window(i0 + 64);
     }
   }
   while (true) {
-    const int len = kv8_len(pos, slots, pg, cap, b), n = (len + kUnit - 1) / kUnit;
-    int u0 = 0, u1 = n, from = 0;
+    int len, slot, u0 = 0, u1, from = 0, n;
     if constexpr (EVEN) {
+      if (b - i0 >= 64) window(i0 + 64);
+      len = __builtin_amdgcn_readlane(lens, b - i0);
+      slot = __builtin_amdgcn_readlane(at_slot, b - i0);
+      n = (len + kUnit - 1) / kUnit;
       if (n == 0) {  // (units are left, so a later row has them)
         ++b;
         continue;
@@ -197,35 +266,39 @@ __global__ void __launch_bounds__(64 * WAVES)
       from = start + kPad;  // of its keys
       u0 = max(at - from, 0), u1 = min(end - from, n);
       if (u1 <= 0) return;  // its keys begin in the next share
+    } else {
+      slot = slots ? slots[b] : b;
+      len = kv8_len(pos[b], slot, pg, cap);
+      n = u1 = (len + kUnit - 1) / kUnit;
     }
-    const int per = (u1 - u0 + WAVES - 1) / WAVES;
-    const int ua = u0 + per * w, ub = min(u1, ua + per);
-    const int slot = slots ? slots[b] : b;
-    u16x8 qf[KS];
-    const uint16_t* qrow = q + ((int64_t)b * Hq + hk * rep + min(c, rep - 1)) * D;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[s] = *reinterpret_cast<const u16x8*>(qrow + chan<D>(s, g));
-      if (c >= rep) qf[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+    Kv8Query<D> qf;
+    qf.load(q + ((int64_t)b * Hq + hk * rep + min(c, rep - 1)) * D, c < rep, g);
     State st;
     st.clear();
-    for (int v0 = ua; v0 < ub; v0 += 64) {
+    for (int v0 = u0; v0 < u1; v0 += 64) {
       // a lane finds one unit: where it lies, and its powers of two (NaN where it lies nowhere)
-      const int m = min(64, ub - v0);
+      const int m = min(64, u1 - v0);
       const int64_t unit = kv8_unit(pg, slot, v0 + min(lane, m - 1), hk);
       const int where = (int)max(unit, (int64_t)0);
-      const float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)pg.ke[where] << 23);
+      const int ke = unit < 0 ? 255 : pg.ke[where];
       const float vs = __uint_as_float((uint32_t)pg.ve[where] << 23);
-      for (int j = 0; j < m; j += 2) {
-        const int j1 = min(j + 1, m - 1);
+      const auto run = [&](auto all, int j) {
+        constexpr bool ALL = decltype(all)::value;
+        const int j1 = ALL ? j + 1 : min(j + 1, m - 1), lim = len - 1 - kUnit * (v0 + j);
         const int64_t a0 = (int64_t)__builtin_amdgcn_readlane(where, j) * (kUnit * D);
         const int64_t a1 = (int64_t)__builtin_amdgcn_readlane(where, j1) * (kUnit * D);
-        const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
-        const int lim = len - 1 - kUnit * (v0 + j);
-        st.take(pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, of(ks, j), of(ks, j1), of(vs, j), of(vs, j1), lim,
-                j1 > j ? lim - kUnit : -1, qf, c, g);
-      }
+        const auto vs_of = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i)); };
+        typename State::Tile t;
+        const int lim1 = j1 > j ? lim - kUnit : -1;
+        State::template load<ALL>(t, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, c, g);
+        __builtin_amdgcn_sched_barrier(0);  // every load is in flight before the first product waits
+        st.template take<ALL>(t, qf, sl, __builtin_amdgcn_readlane(ke, j), __builtin_amdgcn_readlane(ke, j1), vs_of(j),
+                              vs_of(j1), lim, lim1, g);
+      };
+      const int whole = min(m, max(0, len / kUnit - v0));  // units whose rows are all there
+      int j = 2 * w;  // (the waves side by side: 8 x WAVES KB in a row of keys, and of values)
+      for (; j + 2 <= whole; j += 2 * WAVES) run(std::true_type{}, j);
+      for (; j < m; j += 2 * WAVES) run(std::false_type{}, j);
     }
     st.l = lane_sum<32>(lane_sum<16>(st.l));
 #pragma unroll
@@ -265,20 +338,30 @@ __global__ void __launch_bounds__(64 * WAVES)
   }
 }
 
-// the parts of rows that were cut, and the zeros of rows without keys; W: workgroups of a KV head
-template <int D>
-__global__ void __launch_bounds__(D < 64 ? 64 : D)
+// The parts of rows that were cut, and the zeros of rows without keys; W: workgroups of a KV head.  A workgroup has C channels of a
+// row, and G groups of its threads share the parts; a lane has the maximum and the sum of one of 64 parts.  What comes
+// from memory comes at once: the first parts are loaded (where the buffers have room) before they are known to be any.
+template <int D, int C, int G>
+__global__ void __launch_bounds__(C* G)
     kv8_merge_kernel(const float* __restrict__ part_ml, const float* __restrict__ part_o, Kv8Pages pg,
                      const int32_t* __restrict__ pos, const int32_t* __restrict__ slots, uint16_t* __restrict__ out, int B,
                      int Hq, int W, int cap, int nparts) {
-  const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / Hq), d = threadIdx.x, lane = d & 63;
-  const float* ml = part_ml + bh * nparts * 2;
-  const float* po = part_o + bh * nparts * D + min(d, D - 1);
-  const int n = (kv8_len(pos, slots, pg, cap, b) + kUnit - 1) / kUnit;
+  constexpr int AHEAD = G >= 8 ? 2 : G >= 4 ? 3 : 4;
+  __shared__ float sums[G][C];
+  const int64_t bh = blockIdx.x / (D / C);
+  const int b = (int)(bh / Hq), lane = threadIdx.x & 63, grp = threadIdx.x / C;
+  const int d = C * (blockIdx.x % (D / C)) + threadIdx.x % C;
+  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * nparts;
+  const float* po = part_o + bh * nparts * D + d;
+  const float2 first = ml[min(lane, nparts - 1)];
+  float ahead[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) ahead[i] = po[(int64_t)min(grp + i * G, nparts - 1) * D];
+  const auto len = [&](int i) { return kv8_len(pos[i], slots ? slots[i] : i, pg, cap); };
+  const int n = (len(b) + kUnit - 1) / kUnit;
   int total = 0, start = 0;
   for (int i = lane; i < B; i += 64) {
-    const int u = kv8_dealt(pos, slots, pg, cap, i);
+    const int u = kv8_dealt(len(i));
     total += u;
     if (i < b) start += u;
   }
@@ -287,30 +370,109 @@ __global__ void __launch_bounds__(D < 64 ? 64 : D)
   const int parts = n > 0 ? (from + n - 1) / share - from / share + 1 : 0;
   if (parts == 1) return;  // written by its workgroup
   float M = -INFINITY, L = 0.f, acc = 0.f;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, ml[2 * s]);
-  for (int s = 0; s < parts; ++s) {
-    const float m = ml[2 * s], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    L += f * ml[2 * s + 1];
-    acc += f * po[(int64_t)s * D];
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    const bool on = p0 + lane < parts;
+    const float2 x = p0 ? ml[min(p0 + lane, nparts - 1)] : first;
+    const float m = on ? x.x : -INFINITY, top = fmaxf(M, wave_max(m));
+    const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    L = L * was + wave_sum(on ? f * x.y : 0.f);
+    acc *= was;
+    M = top;
+    const int end = min(64, parts - p0);
+    const auto weight = [&](int s) { return __shfl(f, s); };  // (of this wave's groups)
+    int i = 0;
+    if (p0 == 0) {
+#pragma unroll
+      for (; i < AHEAD; ++i) {
+        const int s = grp + i * G;
+        const float wgt = weight(min(s, 63));
+        if (s < end) acc += wgt * ahead[i];
+      }
+    }
+#pragma unroll 8
+    for (; i * G < end; ++i) {  // (every lane takes the same turns)
+      const int s = grp + i * G;
+      const float wgt = weight(min(s, 63)), y = po[(int64_t)(p0 + min(s, end - 1)) * D];
+      if (s < end) acc += wgt * y;
+    }
   }
-  if (d < D) out[bh * D + d] = f2bf(L == 0.f ? 0.f : acc / L);
+  if constexpr (G > 1) {
+    sums[grp][threadIdx.x % C] = acc;
+    __syncthreads();
+    if (threadIdx.x >= C) return;
+    acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) acc += sums[i][threadIdx.x];
+  }
+  out[bh * D + d] = f2bf(L == 0.f ? 0.f : acc / L);
 }
 
 }  // namespace mx
 
 using namespace mx;
 
+// Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 6 us for 256 KB (43 GB/s a CU, whatever
+// its waves); cutting costs a merge and more ends, 4 to 9 us.  Us with whole rows of 4 / 8 / 16 waves, and cut:
+//   1 x 700 keys, 8 heads of 64 5.6 / 5.2 / 5.6, 7.7; of 128 8.3 / 8.0 / 8.0, 9.4; 1 x 4096 of 128 27 / 26 / 26, 11.6
+//   16 x 500 .. 2000, 8 heads of 64 12.2 / 9.6 / 9.1, 12.6;  40 x 1000 .. 4000, 5 heads of 64 22.5 / 17.1 / 15.9, 18.8
+//   32 x 100 .. 2000, 8 heads of 128 20.1 / 17.6 / 17.3, 23.6;  64 x 2048 .. 4096 77.3 / 80.9 / 85.1, 86.7
+// Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 10 us.
+static int kv8_waves(int64_t rows, int64_t cap, int D) {
+  const int64_t bytes = cap * D;  // of keys
+  if (bytes > (rows >= 384 ? 524288 : rows >= 128 ? 262144 : 131072)) return 0;
+  return rows >= 384 ? 4 : rows >= 96 ? 16 : 8;
+}
 // workgroups of a KV head where keys are dealt evenly: two a CU of 256
 static int kv8_shares(int Hkv) { return Hkv < 512 ? (512 + Hkv - 1) / Hkv : 1; }
-// whether a workgroup takes a whole row: up to 512 keys, where a launch to merge would cost more than it saves
-static bool kv8_whole(int cap) { return cap <= 512; }
 
-// parts that a row of up to `cap` keys can be cut into (of part_ml [B, Hq, parts, 2], part_o [B, Hq, parts, D])
-extern "C" int mx_kv8_attn_parts(int Hkv, int cap) {
-  if (kv8_whole(cap)) return 0;
+// parts that a row of up to `cap` keys can be cut into (of part_ml [B, Hq, parts, 2], part_o [B, Hq, parts, D]); 0: rows are whole
+extern "C" int mx_kv8_attn_parts(int B, int Hkv, int D, int cap) {
+  if (kv8_waves((int64_t)B * Hkv, cap, D)) return 0;
   const int W = kv8_shares(Hkv), most = (cap / kUnit + 1) / kLeast + 2;
   return W < most ? W : most;
 }
+
+namespace {
+
+struct Launch {
+  const uint16_t* q;
+  Kv8Pages pg;
+  const int32_t *pos, *slots;
+  float *part_ml, *part_o;
+  uint16_t* out;
+  int B, Hq, cap;
+  float sl;
+  hipStream_t stream;
+};
+
+template <int D, int WAVES>
+void launch_whole(const Launch& a) {
+  kv8_attn_kernel<D, WAVES, false><<<dim3(a.pg.Hkv, a.B), 64 * WAVES, 0, a.stream>>>(
+      a.q, a.pg, a.pos, a.slots, nullptr, nullptr, a.out, a.B, a.Hq, a.cap, 0, a.sl);
+}
+
+template <int D>
+void launch(const Launch& a) {
+  const int Hkv = a.pg.Hkv, nparts = mx_kv8_attn_parts(a.B, Hkv, D, a.cap), W = kv8_shares(Hkv);
+  if (!nparts) {
+    const int waves = kv8_waves((int64_t)a.B * Hkv, a.cap, D);
+    if (waves == 4) launch_whole<D, 4>(a);
+    else if (waves == 8) launch_whole<D, 8>(a);
+    else launch_whole<D, 16>(a);
+    return;
+  }
+  kv8_attn_kernel<D, 4, true><<<dim3(W, Hkv), 256, 0, a.stream>>>(a.q, a.pg, a.pos, a.slots, a.part_ml, a.part_o, a.out,
+                                                                  a.B, a.Hq, a.cap, nparts, a.sl);
+  const int rows = a.B * a.Hq;
+  if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.1 -> 10.4 us, 1 x 32768 34.9 -> 19.9
+    kv8_merge_kernel<D, 32, 8><<<rows * (D / 32), 256, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots, a.out, a.B,
+                                                                      a.Hq, W, a.cap, nparts);
+  else
+    kv8_merge_kernel<D, D, D < 128 ? 128 / D : 1><<<rows, 128, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots,
+                                                                              a.out, a.B, a.Hq, W, a.cap, nparts);
+}
+
+}  // namespace
 
 // q [B, Hq, D]; keys 0 .. pos[b], below cap, of slot slots[b] (null: b); out [B, Hq, D]
 extern "C" int mx_kv8_attn(const uint16_t* q, const Kv8Pages* cache, const int32_t* pos, const int32_t* slots,
@@ -319,26 +481,12 @@ extern "C" int mx_kv8_attn(const uint16_t* q, const Kv8Pages* cache, const int32
   if (B <= 0) return 0;
   const Kv8Pages pg = *cache;
   if (pg.Hkv <= 0 || Hq % pg.Hkv || Hq / pg.Hkv > 16 || B > 65535 || pg.Hkv > 65535 || cap < 1 ||
-      (int64_t)B * (cap / kUnit + 1 + kPad) > INT32_MAX)
+      (int64_t)B * (cap / kUnit + 1 + kPad) > INT32_MAX || (int64_t)B * Hq * (D / 32) > INT32_MAX || !(scale > 0.f))
     return -1;
-  const float sl = scale * 1.4426950408889634f;
-  const int nparts = mx_kv8_attn_parts(pg.Hkv, cap), W = kv8_shares(pg.Hkv);
-#define ATTN(DD)                                                                                                         \
-  do {                                                                                                                   \
-    if (kv8_whole(cap)) {                                                                                                \
-      kv8_attn_kernel<DD, 8, false><<<dim3(pg.Hkv, B), 512, 0, stream>>>(q, pg, pos, slots, nullptr, nullptr, out, B,    \
-                                                                         Hq, cap, 0, sl);                                \
-    } else {                                                                                                             \
-      kv8_attn_kernel<DD, 4, true><<<dim3(W, pg.Hkv), 256, 0, stream>>>(q, pg, pos, slots, part_ml, part_o, out, B, Hq,  \
-                                                                        cap, nparts, sl);                                \
-      kv8_merge_kernel<DD><<<B * Hq, DD < 64 ? 64 : DD, 0, stream>>>(part_ml, part_o, pg, pos, slots, out, B, Hq, W,     \
-                                                                     cap, nparts);                                       \
-    }                                                                                                                    \
-  } while (0)
-  if (D == 128) ATTN(128);
-  else if (D == 64) ATTN(64);
-  else if (D == 32) ATTN(32);
+  const Launch a{q, pg, pos, slots, part_ml, part_o, out, B, Hq, cap, scale * 1.4426950408889634f, stream};
+  if (D == 128) launch<128>(a);
+  else if (D == 64) launch<64>(a);
+  else if (D == 32) launch<32>(a);
   else return -1;
-#undef ATTN
   return (int)hipGetLastError();
 }

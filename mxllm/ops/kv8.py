@@ -158,15 +158,15 @@ def decode_attention(q: torch.Tensor, pages: Pages, pos: torch.Tensor, slots: to
                      scale: float | None = None) -> torch.Tensor:
     """One token of each sequence: q [B, Hq, D] over positions 0 .. pos[b] of slot slots[b] (int32 [B]; None: the rows'
     numbers) -> [B, Hq * D].  ``max_len`` >= 1 bounds the positions that any row looks at (a host number, for the launch;
-    positions at it and behind are not seen).  A row without keys (pos < 0, or a slot that is none) gives zeros."""
+    positions at it and behind are not seen), ``scale`` > 0.  A row without keys (pos < 0, or a slot that is none) gives zeros."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if use_native(q):
         return native().kv8_decode_attn(q.contiguous(), *pages, pos, slots, max_len, scale)
     _check_pages(pages)
     B, Hq, D = q.shape
     Hkv = pages.k.shape[1]
-    if D != pages.k.shape[3] or Hq % Hkv or max_len < 1:
-        raise ValueError(f"q {tuple(q.shape)} over a cache of {Hkv} heads of {pages.k.shape[3]}, max_len {max_len}")
+    if D != pages.k.shape[3] or Hq % Hkv or max_len < 1 or not 0 < scale < math.inf:
+        raise ValueError(f"q {tuple(q.shape)} over a cache of {Hkv} heads of {pages.k.shape[3]}, max_len {max_len}, scale {scale}")
     _check_ints(pos, (B,), "pos")
     cap = min(max_len, pages.table.shape[1] * pages.k.shape[2])
     out = torch.zeros(B, Hq, D)

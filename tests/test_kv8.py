@@ -151,6 +151,9 @@ def test_refusals():
         kv8.decode_attention(torch.zeros(2, 2, D), p, i32, i32, 0)
     with pytest.raises(ValueError):
         kv8.decode_attention(torch.zeros(2, 2, 64), p, i32, i32, 8)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            kv8.decode_attention(torch.zeros(2, 2, D), p, i32, i32, 8, scale)
     with pytest.raises(ValueError):
         kv8.Pages.empty(2, 1, 24, D, p.table)
     for starts, lens, slots in [([0], [1, 2], [0]), ([0, 4], [1, 2], [3, 3]), ([-1], [2], [0]), ([0], [-2], [0])]:

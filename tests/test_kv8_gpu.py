@@ -220,6 +220,25 @@ def test_attention_of_long_and_uneven_rows(gpu, D, Hq, Hkv, lens):
     _check_attention(gpu, lens, Hq, Hkv, 256, D, seed=len(lens))
 
 
+@pytest.mark.parametrize("B,hi", [(64, 700), (64, 2100), (20, 900), (130, 1000)])
+def test_attention_of_whole_rows_of_4_8_and_16_waves(gpu, B, hi):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, hi, (B,), generator=g).tolist()
+    _check_attention(gpu, lens + [hi], 16, 8, 256, 64, seed=B)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -60, 1.0, 2.0 ** 60])
+def test_queries_of_unlike_sizes(gpu, size):
+    """Channels of a query from 2^-14 of its largest on, whose low codes end, and queries far from one."""
+    D, Hq, Hkv = 128, 8, 2
+    p = _random_pages(gpu, [600, 2000], Hkv, 256, D)
+    q = (torch.randn(2, Hq, D, device=gpu) * 2.0 ** torch.randint(-14, 1, (2, Hq, D), device=gpu).float()).bfloat16()
+    q[0, 3] = 0
+    got = kv8.decode_attention(q * size, p, _i32([599, 1999], gpu), None, 2000, D ** -0.5 / size).view(2, Hq, D)
+    want, total = _exact(q, p, [599, 1999], [0, 1], 2000, D ** -0.5)
+    assert bool(((got.double().cpu() - want).abs() <= (HALF + 2.0 ** -11) * total + HALF * want.abs()).all())
+
+
 def test_attention_of_many_rows_one_slot_and_small_pages(gpu):
     _check_attention(gpu, [700, 33, 2100], 32, 8, 16, 64, order=[0, 1, 2, 2, 0, 1, 0] * 40)
 
@@ -337,7 +356,8 @@ def test_refusals(gpu):
             kv8.append_prompts(rows, cos, sin, runs, p, Hq)
     q = torch.zeros(2, Hq, D, device=gpu, dtype=torch.bfloat16)
     for args in [(q.float(), p, i32, i32, 8), (q, p, i32, i32, 0), (q[:, :3], p, i32, i32, 8), (q[..., :32], p, i32, i32, 8), (q[:1], p, i32, i32, 8),
-                 (torch.zeros(2, 34, D, device=gpu, dtype=torch.bfloat16), p, i32, i32, 8), (q, p, i32.long(), i32, 8)]:
+                 (torch.zeros(2, 34, D, device=gpu, dtype=torch.bfloat16), p, i32, i32, 8), (q, p, i32.long(), i32, 8),
+                 (q, p, i32, i32, 8, 0.0), (q, p, i32, i32, 8, -0.1), (q, p, i32, i32, 8, math.nan), (q, p, i32, i32, 8, math.inf)]:
         with pytest.raises(RuntimeError):
             kv8.decode_attention(*args)
     with pytest.raises(RuntimeError):
