@@ -4,12 +4,12 @@
 // Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
 // group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 55 us, where loads alone take 53 and a linear read of as much 45.
 //
-// Scores by v_mfma_scale_f32_16x16x128_f8f6f4 on the codes themselves: keys as they lie, under their unit's (16 positions)
-// exponent byte, queries as sums of two e4m3 codes (Kv8Query).  Codes as bf16 cost 32 conversions a tile and the query's
-// products nothing less: 40 x 1000 .. 4000 keys of 64 18.1 -> 16.2 us, 64 x 30 .. 512 of 128 13.5 -> 11.1, long ones alike.
-//   S^T[key][head] = 2^(ek - 127) 2^(eq - 127) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
-// The outputs by v_mfma_f32_16x16x32_bf16: values become bf16 in registers, where they are exact, and a weight is rounded
-// once to bf16 (2^-8 of it, in a sum of many), while the sum under it takes what was not rounded.  Sums and outputs are f32.
+//   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
+// by v_mfma_f32_16x16x32_bf16 on codes that become bf16 in registers, where they are exact, the units' (16 positions) powers of
+// two in the scores and in the conversion of values.  Sums and outputs are f32; a weight is rounded once to bf16 (2^-8 of
+// it, in a sum of many), while the sum under it takes what was not rounded.  (Scores on the codes themselves, queries as
+// sums of two e4m3 codes under v_mfma_scale_f32_16x16x128_f8f6f4, save 32 conversions a tile and no time, and that
+// product drops what is 2^-13 of its largest summand: outputs 2.3e-3 off in place of 2.0e-3.)
 //
 // The operands: a lane (c, g) of K has row c of a unit and the channels 64 h + 16 g .. + 15 (a dot product does not mind the
 // order, so a lane takes whole pieces of 16 bytes; queries are laid out alike), of V eight rows and D / 16 neighbouring
@@ -25,16 +25,11 @@
 namespace mx {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4v& a, const u16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
-}
-// codes a under 2^(ea - 127) (one of each row), codes b under 2^(eb - 127) (one of each column)
-__device__ __forceinline__ f32x4 mfma128(const i32x8& a, const i32x8& b, const f32x4& c, int ea, int eb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, ea, 0, eb);
 }
 __device__ __forceinline__ uint32_t pair_bf16(uint32_t w, float scale, bool high) {
   return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
@@ -57,52 +52,15 @@ __device__ __forceinline__ uint32_t word(uint2 v, int i) { return i ? v.y : v.x;
 __device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
 __device__ __forceinline__ uint32_t word(uint16_t v, int) { return v; }
 
-// A head's query as codes: high, the nearest e4m3 of q 2^s, and low, the nearest of what is left, s such that the largest channel
-// is in [128, 256).  A bf16 number is their sum exactly where it is at least 2^-10 of the largest channel, and off by 2^-18 of
-// that below.  Laid out as the lane (c, g) has its channels of a key: head c.
+// channel of k-step s of lane group g
 template <int D>
-struct Kv8Query {
-  static constexpr int PARTS = D == 128 ? 2 : 1;  // products a unit: high and low in one where a head leaves room
-  i32x8 q[PARTS];
-  int e;  // its power of two
-
-  __device__ __forceinline__ void load(const uint16_t* row, bool on, int g) {
-    constexpr int N = D / 4;  // channels of a lane
-    float x[N];
-    float top = 0.f;
-#pragma unroll
-    for (int h = 0; h < N / 8; ++h) {
-      const u16x8 v = *reinterpret_cast<const u16x8*>(row + (D == 32 ? 8 * g : 64 * (h >> 1) + 16 * g + 8 * (h & 1)));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[8 * h + j] = on ? bf2f(v[j]) : 0.f;
-        top = fmaxf(top, fabsf(x[8 * h + j]));
-      }
-    }
-    top = lane_max<32>(lane_max<16>(top));
-    e = max((int)(__float_as_uint(top) >> 23), 8) - 7;  // (2^-120 and less: as codes of 2^-120)
-    uint32_t hi[N / 4], lo[N / 4];
-#pragma unroll
-    for (int w = 0; w < N / 4; ++w) {
-      hi[w] = kv8_code4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3], 127 - e);
-      float y[4];
-      kv8_value4(hi[w], e - 127, y);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = x[4 * w + j] - y[j];
-      lo[w] = kv8_code4(y[0], y[1], y[2], y[3], 127 - e);
-    }
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if constexpr (D == 128) q[0][w] = hi[w], q[1][w] = lo[w];
-      else if constexpr (D == 64) q[0][w] = w < 4 ? hi[w & 3] : lo[w & 3];
-      else q[0][w] = w < 2 ? hi[w & 1] : w < 4 ? lo[w & 1] : 0;
-    }
-  }
-};
+__device__ __forceinline__ int chan(int s, int g) {
+  return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+}
 
 template <int D>
 struct Kv8State {  // of one wave
-  static constexpr int E = D / 16, KW = D / 16;  // channels of V and words of K that a lane has of a row
+  static constexpr int E = D / 16, KS = D / 32;
   float m, l;   // reference of the exponents of head c; l: this lane's keys
   f32x4 o[E];   // [e][i]: channel E (4 g + i) + e of head c
 
@@ -114,7 +72,7 @@ struct Kv8State {  // of one wave
 
   // two units of one wave, on their way from memory
   struct Tile {
-    uint32_t k[2][KW];
+    uint32_t k[2][2 * KS];          // words of the lane's channels, in the order of the k-steps
     typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
   };
   // k0, v0 / k1, v1: the units; ALL: every row of both is there; else lim: their last one (less than 0: none), and rows behind it
@@ -145,28 +103,29 @@ struct Kv8State {  // of one wave
     }
   }
 
-  // ke: exponent bytes of the units' keys, vs: powers of two of their values
+  // ks: what the units' scores are multiplied by, vs: powers of two of their values
   template <bool ALL>
-  __device__ __forceinline__ void take(const Tile& t, const Kv8Query<D>& qf, float sl, int ke0, int ke1, float vs0, float vs1,
+  __device__ __forceinline__ void take(const Tile& t, const u16x8 (&qf)[KS], float ks0, float ks1, float vs0, float vs1,
                                        int lim0, int lim1, int g) {
     f32x4 sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      i32x8 a;
+      sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 8; ++w) a[w] = (int)t.k[j][w % KW];
-      const int ke = j ? ke1 : ke0;
-      sc[j] = mfma128(a, qf.q[0], f32x4{0.f, 0.f, 0.f, 0.f}, ke, qf.e);
-      if constexpr (Kv8Query<D>::PARTS > 1) sc[j] = mfma128(a, qf.q[1], sc[j], ke, qf.e);
-      if (!ALL) {
+      for (int s = 0; s < KS; ++s)
+        sc[j] = mfma16(__builtin_bit_cast(u32x4v, dequant8(t.k[j][2 * s], t.k[j][2 * s + 1])), qf[s], sc[j]);
+    }
+    float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[j][i] = 4 * g + i <= (j ? lim1 : lim0) ? sc[j][i] : -INFINITY;
-      }
+    for (int i = 0; i < 8; ++i) {
+      x[i] = sc[i >> 2][i & 3] * (i < 4 ? ks0 : ks1);
+      if (!ALL) x[i] = 4 * g + (i & 3) <= (i < 4 ? lim0 : lim1) ? x[i] : -INFINITY;
     }
     // The exponents' reference is a maximum that may be behind by 2^8: weights up to there cost no precision, and the sums are
     // multiplied again in a few of the tiles only
-    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                      fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl;
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
     if (__ballot(top > m + 8.f)) {
       const float now = fmaxf(m, lane_max<32>(lane_max<16>(top))), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
       m = now;
@@ -177,13 +136,11 @@ struct Kv8State {  // of one wave
     const float mref = m == -INFINITY ? 0.f : m;
     u16x8 pb;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], sl, -mref));
-        l += p;
-        pb[4 * j + i] = f2bf(p);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float p = __builtin_amdgcn_exp2f(x[i] - mref);
+      l += p;
+      pb[i] = f2bf(p);
+    }
     // bytes 0, 1 or 2, 3 of the words of two rows side by side, as pairs of rows of one channel each
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
@@ -216,7 +173,7 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
                     const int32_t* __restrict__ slots, float* __restrict__ part_ml, float* __restrict__ part_o,
                     uint16_t* __restrict__ out, int B, int Hq, int cap, int nparts, float sl) {
   typedef Kv8State<D> State;
-  constexpr int E = State::E, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
+  constexpr int E = State::E, KS = State::KS, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
   typedef float orow_t __attribute__((ext_vector_type(E)));
   __shared__ __attribute__((aligned(32))) float so[WAVES * 16 * ROW];
   __shared__ float mls[WAVES][2][16];
@@ -271,8 +228,13 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
       len = kv8_len(pos[b], slot, pg, cap);
       n = u1 = (len + kUnit - 1) / kUnit;
     }
-    Kv8Query<D> qf;
-    qf.load(q + ((int64_t)b * Hq + hk * rep + min(c, rep - 1)) * D, c < rep, g);
+    u16x8 qf[KS];
+    const uint16_t* qrow = q + ((int64_t)b * Hq + hk * rep + min(c, rep - 1)) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = *reinterpret_cast<const u16x8*>(qrow + chan<D>(s, g));
+      if (c >= rep) qf[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
     State st;
     st.clear();
     for (int v0 = u0; v0 < u1; v0 += 64) {
@@ -280,20 +242,18 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
       const int m = min(64, u1 - v0);
       const int64_t unit = kv8_unit(pg, slot, v0 + min(lane, m - 1), hk);
       const int where = (int)max(unit, (int64_t)0);
-      const int ke = unit < 0 ? 255 : pg.ke[where];
+      const float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)pg.ke[where] << 23);
       const float vs = __uint_as_float((uint32_t)pg.ve[where] << 23);
       const auto run = [&](auto all, int j) {
         constexpr bool ALL = decltype(all)::value;
-        const int j1 = ALL ? j + 1 : min(j + 1, m - 1), lim = len - 1 - kUnit * (v0 + j);
+        const int j1 = ALL ? j + 1 : min(j + 1, m - 1), lim = len - 1 - kUnit * (v0 + j), lim1 = j1 > j ? lim - kUnit : -1;
         const int64_t a0 = (int64_t)__builtin_amdgcn_readlane(where, j) * (kUnit * D);
         const int64_t a1 = (int64_t)__builtin_amdgcn_readlane(where, j1) * (kUnit * D);
-        const auto vs_of = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i)); };
+        const auto of = [](float x, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
         typename State::Tile t;
-        const int lim1 = j1 > j ? lim - kUnit : -1;
         State::template load<ALL>(t, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, c, g);
         __builtin_amdgcn_sched_barrier(0);  // every load is in flight before the first product waits
-        st.template take<ALL>(t, qf, sl, __builtin_amdgcn_readlane(ke, j), __builtin_amdgcn_readlane(ke, j1), vs_of(j),
-                              vs_of(j1), lim, lim1, g);
+        st.template take<ALL>(t, qf, of(ks, j), of(ks, j1), of(vs, j), of(vs, j1), lim, lim1, g);
       };
       const int whole = min(m, max(0, len / kUnit - v0));  // units whose rows are all there
       int j = 2 * w;  // (the waves side by side: 8 x WAVES KB in a row of keys, and of values)
