@@ -49,6 +49,7 @@ def main(argv=None) -> dict:
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--kv-pool-tokens", type=int, default=None,
                     help="paged KV cache shared by all slots (default: every slot owns max_seq positions)")
+    ap.add_argument("--kv-dtype", choices=["bf16", "e4m3"], default=None, help="e4m3: keys and values in 8 bits")
     ap.add_argument("--tp-shard-proxy", type=int, default=0,
                     help="one GPU: run rank 0's TP-N shard without the collectives (per-GPU compute floor)")
     a = ap.parse_args(argv)
@@ -91,7 +92,8 @@ def main(argv=None) -> dict:
         sum(b.numel() * b.element_size() for n, b in model.named_buffers() if n.endswith((".q", ".scale")))
     bmax = max(int(b) for b in a.batches.split(","))
     max_seq = max(a.prompt_len, a.ctx + a.decode_steps, a.e2e_prompt_len + a.new_tokens) + 8
-    eng = Engine(model, max_batch=max(bmax, 1), max_seq=max_seq, tp_group=tp_group, kv_pool_tokens=a.kv_pool_tokens)
+    eng = Engine(model, max_batch=max(bmax, 1), max_seq=max_seq, tp_group=tp_group, kv_pool_tokens=a.kv_pool_tokens,
+                 kv_dtype=a.kv_dtype)
     g = torch.Generator().manual_seed(0)
 
     def prompt(n):

@@ -234,9 +234,34 @@ at::Tensor kv8_decode_attn(const at::Tensor& q, const at::Tensor& kc, const at::
   return out;
 }
 
+// causal attention inside each segment of blocks [n, 4] (mxllm/ops/hybrid.py PromptRows.attn_blocks): q [Hq, T, D], k, v
+// [Hkv, T, D] -> [T, Hq * D]
+at::Tensor prompt_rows_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& blocks,
+                                 double scale) {
+  check_bf16(q, "q");
+  check_bf16(k, "k");
+  check_bf16(v, "v");
+  MX_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == q.size(1) && k.size(2) == q.size(2) &&
+               k.device() == q.device() && v.device() == q.device(),
+           "q [Hq, T, D], k, v [Hkv, T, D] on one device");
+  const int64_t Hq = q.size(0), T = q.size(1), D = q.size(2), Hkv = k.size(0);
+  check_heads(Hq, Hkv, D);
+  MX_CHECK(T * D * 2 < INT32_MAX, "prompt_rows_attention: too many rows");
+  MX_CHECK(blocks.dim() == 2, "blocks int32 [n, 4]");
+  const int32_t* bl = check_ints(blocks, {blocks.size(0), 4}, q, "blocks");
+  DevGuard g(q.device());
+  auto o = at::empty({T, Hq * D}, q.options());
+  const int rc = mx_attn_fwd_prompts(bf(q), bf(k), bf(v), bl, (int)blocks.size(0), bfm(o), (int)T, (int)Hq, (int)Hkv, (int)D,
+                                     (float)scale, cur_stream());
+  MX_CHECK(rc != -1, "prompt_rows_attention: sizes not taken");
+  MX_OK(rc);
+  return o;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mxllm, m) {
+  m.def("prompt_rows_attention(Tensor q, Tensor k, Tensor v, Tensor blocks, float scale) -> Tensor");
   m.def("qk_norm_rope(Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int B, int S, int Hq, int Hkv, int D, float eps, Tensor? positions=None) -> (Tensor, Tensor, Tensor)");
   m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor dv, Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int Hkv, float eps, Tensor? positions=None, int out_pad=0, bool need_dw=True, bool dw32=False) -> (Tensor, Tensor, Tensor)");
   m.def("kv8_append_tokens(Tensor qkv, Tensor cos, Tensor sin, Tensor pos, Tensor? slots, Tensor(a!) k, Tensor(b!) v, Tensor(c!) ke, Tensor(d!) ve, Tensor table, int Hq, Tensor? wq, Tensor? wk, float eps) -> Tensor");
@@ -250,6 +275,7 @@ TORCH_LIBRARY_IMPL(mxllm, CUDA, m) {
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.impl("kv8_append_tokens", &kv8_append_tokens);
   m.impl("kv8_append_prompts", &kv8_append_prompts);
+  m.impl("prompt_rows_attention", &prompt_rows_attention);
   m.impl("kv8_read", &kv8_read);
   m.impl("kv8_decode_attn", &kv8_decode_attn);
 }

@@ -135,6 +135,21 @@ def append_prompts(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, runs
     return tuple(x.transpose(0, 1).contiguous().to(qkv.dtype) for x in (q, k, v))
 
 
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: list[int],
+                     blocks: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of each of several prompts to itself: q [Hq, T, D], k, v [Hkv, T, D] of sequences of ``lens`` rows one
+    after another (``append_prompts`` from position 0) -> [T, Hq * D].  ``blocks``: the table of 128-row blocks
+    (``PromptRows.attn_blocks(max(lens))``), which the GPU needs."""
+    if use_native(q):
+        return native().prompt_rows_attention(q, k, v, blocks, 1.0 / math.sqrt(q.shape[-1]))
+    out, at = [], 0
+    for n in lens:
+        o = ref.attention(*(x[None, :, at:at + n].transpose(1, 2) for x in (q, k, v)))
+        out.append(o.reshape(n, -1))
+        at += n
+    return torch.cat(out)
+
+
 def read(pages: Pages, slots: torch.Tensor | None, starts: torch.Tensor, ends: torch.Tensor, n: int):
     """(k, v) bf16 [B, Hkv, n, D] of positions starts[b] + i, i < n, of slot slots[b] (int32 [B]); zero from ends[b] on.
     Exact: bf16 holds every value of the cache (under exponent bytes of 3 and more)."""

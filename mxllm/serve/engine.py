@@ -84,13 +84,16 @@ class Request:
 class Engine:
     def __init__(self, model, max_batch: int = 8, max_seq: int = 4096, device=None, eos_ids=(),
                  use_graphs: bool | None = None, prefill_tokens: int = 16384, tp_group=None,
-                 kv_pool_tokens: int | None = None, kv_block: int = 256):
+                 kv_pool_tokens: int | None = None, kv_block: int = 256, kv_dtype: str | None = None):
         """``tp_group``: serve a tensor-parallel shard (mxllm/parallel/tensor.py
         ``shard_llama`` / ``random_shard``) with the other ranks of the group;
         every rank of the group runs the same schedule (same submissions in the
         same order, e.g. SPMD ``generate`` or ``serve_follower``).
         ``kv_pool_tokens``: paged KV cache of that many tokens shared by all slots
-        (None: every slot owns max_seq positions; env MXLLM_KV_POOL_TOKENS)."""
+        (None: every slot owns max_seq positions; env MXLLM_KV_POOL_TOKENS).
+        ``kv_dtype``: "bf16" (the model's type) or "e4m3", keys and values in 8 bits with a power of two for each 16
+        positions of a head (mxllm/ops/kv8.py): twice the positions in the same memory, and half the bytes a decode step
+        reads of them (env MXLLM_KV_DTYPE; Llama models)."""
         self.model = model
         self.tp = None
         if tp_group is not None:
@@ -126,6 +129,9 @@ class Engine:
         n_slots = max_batch + (1 if self.use_graphs else 0)
         if kv_pool_tokens is None and os.environ.get("MXLLM_KV_POOL_TOKENS"):
             kv_pool_tokens = int(os.environ["MXLLM_KV_POOL_TOKENS"])
+        self.kv_dtype = kv_dtype or os.environ.get("MXLLM_KV_DTYPE") or "bf16"
+        if self.kv_dtype not in ("bf16", "e4m3"):
+            raise ValueError(f"kv_dtype {self.kv_dtype!r}: bf16 or e4m3")
         from .steps import steps_for
 
         self.model_steps = steps_for(model)(self)

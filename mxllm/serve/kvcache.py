@@ -25,6 +25,8 @@ One spare slot with one block takes the padding rows of a graphed decode step.
 row p % (that layer's run); a slot then needs blocks for ``span`` (the longest run) positions
 only, however long its sequence grows.
 
+``KV8Cache`` is the same with keys and values in 8 bits.
+
 ``StateCache`` holds what a slot keeps at a fixed size: recurrent state (f32), the last inputs
 of short convolutions, and the last rows of windowed layers beside layers that keep all positions.
 """
@@ -33,6 +35,8 @@ from __future__ import annotations
 import math
 
 import torch
+
+from ..ops import kv8
 
 BLOCK = 256
 
@@ -175,6 +179,32 @@ class KVCache:
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.k + self.v)
+
+
+class KV8Cache(KVCache):
+    """Keys and values as e4m3 codes with a power of two for each 16 positions of a head (mxllm/ops/kv8.py): half of what
+    bf16 takes, in blocks and tables of the same kind.  ``pages(layer)`` is what the operators take."""
+
+    def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, device, n_slots: int, max_seq: int,
+                 pool_tokens: int | None = None, block: int = BLOCK, scratch_slot: int | None = None):
+        super().__init__(n_layers, n_kv_heads, head_dim, torch.uint8, device, n_slots, max_seq, pool_tokens, block, scratch_slot)
+        shape = (self.n_blocks, n_kv_heads, block // kv8.GROUP)
+        self.k_exp, self.v_exp = ([torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(n_layers)] for _ in range(2))
+
+    def pages(self, layer: int) -> kv8.Pages:
+        return kv8.Pages(self.k[layer], self.v[layer], self.k_exp[layer], self.v_exp[layer], self.bt)
+
+    def write(self, layer: int, slot: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        raise NotImplementedError("an 8-bit cache is appended to (mxllm.ops.kv8), which rounds keys and values once")
+
+    def gather(self, layer: int, slot: int, L: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The values of positions [0, L) of ``slot`` as bf16 [Hkv, L, D]."""
+        at = torch.tensor([[slot], [0], [L]], dtype=torch.int32, device=self.bt.device)
+        k, v = kv8.read(self.pages(layer), at[0], at[1], at[2], L)
+        return k[0], v[0]
+
+    def nbytes(self) -> int:
+        return super().nbytes() + sum(t.numel() for t in self.k_exp + self.v_exp)
 
 
 class StateCache:

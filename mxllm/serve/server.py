@@ -204,8 +204,8 @@ def build_app(engine: Engine, tokenizer, model_name: str, api_key: str | None = 
 
 def build_default(model: str = "tiny", device: str | None = None, max_batch: int = 8, max_seq: int = 2048,
                   checkpoint: str | None = None, tokenizer_path: str | None = None, seed: int = 0,
-                  weights: str = "bf16", tp_group=None):
-    """Engine + tokenizer.  ``tp_group``: this rank serves its tensor-parallel
+                  weights: str = "bf16", tp_group=None, kv_dtype: str | None = None):
+    """Engine + tokenizer.  ``kv_dtype``: the engine's.  ``tp_group``: this rank serves its tensor-parallel
     shard (mxllm/parallel/tensor.py) of the model; the full model is built (or
     loaded) on the rank's GPU, sliced and freed."""
     from ..data.tokenizer import get_tokenizer
@@ -236,7 +236,7 @@ def build_default(model: str = "tiny", device: str | None = None, max_batch: int
         quantize_model_fp8_(m)
     tok = get_tokenizer(cfg.vocab_size, tokenizer_path, cfg.bos_id, cfg.eos_id)
     eng = Engine(m, max_batch=max_batch, max_seq=max_seq, eos_ids=(cfg.eos_id, getattr(tok, "eos_id", cfg.eos_id)),
-                 tp_group=tp_group)
+                 tp_group=tp_group, kv_dtype=kv_dtype)
     return eng, tok
 
 
@@ -255,6 +255,8 @@ def main(argv=None):
     ap.add_argument("--served-name", default=None)
     ap.add_argument("--weights", choices=["bf16", "fp8"], default=os.environ.get("MXLLM_ENGINE_WEIGHTS", "bf16"),
                     help="fp8: e4m3 projection weights (serving quantisation, mxllm/serve/quant.py)")
+    ap.add_argument("--kv-dtype", choices=["bf16", "e4m3"], default=None,
+                    help="e4m3: keys and values in 8 bits (mxllm/ops/kv8.py; default: MXLLM_KV_DTYPE, else bf16)")
     ap.add_argument("--tp", type=int, default=1,
                     help="tensor-parallel degree: launch with torchrun --nproc-per-node=TP; rank 0 serves HTTP, "
                          "the other ranks follow its schedule")
@@ -271,7 +273,7 @@ def main(argv=None):
             raise SystemExit(f"--tp {a.tp} needs exactly {a.tp} ranks (torchrun --nproc-per-node={a.tp})")
         group = dist.group.WORLD
     eng, tok = build_default(a.model, None, a.max_batch, a.max_seq, a.checkpoint, a.tokenizer, weights=a.weights,
-                             tp_group=group)
+                             tp_group=group, kv_dtype=a.kv_dtype)
     if group is not None:
         eng.enable_tp_sync()
         if env.rank != 0:

@@ -24,9 +24,10 @@ from ..models.llama import FusedLinear, Llama, hooked
 from ..models.revesun import Revesun
 from ..models.sigusun import Sigusun
 from ..ops import decode as dops
+from ..ops import kv8
 from ..ops.hybrid import PromptRows, SeqCaches, TokenRows
 from ..ops.latent import LatentCache
-from .kvcache import KVCache, StateCache
+from .kvcache import KV8Cache, KVCache, StateCache
 from .quant import W8Linear
 
 _SWIGLU_FUSED = os.environ.get("MXLLM_SWIGLU_FUSED", "1") != "0"  # A/B switch (bench/serve_bench.py)
@@ -51,9 +52,16 @@ class LlamaSteps:
 
     def make_cache(self, n_slots: int, pool_tokens: int | None, block: int) -> KVCache:
         eng, c = self.eng, self.cfg
-        kv = KVCache(c.n_layers, c.n_kv_heads, c.head_dim, self.model.tok_emb.dtype, eng.device, n_slots, eng.max_seq,
-                     pool_tokens=pool_tokens, block=block,
-                     scratch_slot=eng.scratch_slot if eng.use_graphs else None)
+        scratch = eng.scratch_slot if eng.use_graphs else None
+        self.kv8 = eng.kv_dtype == "e4m3"
+        if self.kv8:
+            if eng.device.type == "cuda" and (c.head_dim not in (32, 64, 128) or c.n_heads // c.n_kv_heads > 16):
+                raise ValueError(f"kv_dtype e4m3: heads of 32, 64 or 128 channels, up to 16 a key head, not {c.head_dim}, "
+                                 f"{c.n_heads // c.n_kv_heads}")
+            kv = KV8Cache(c.n_layers, c.n_kv_heads, c.head_dim, eng.device, n_slots, eng.max_seq, pool_tokens, block, scratch)
+        else:
+            kv = KVCache(c.n_layers, c.n_kv_heads, c.head_dim, self.model.tok_emb.dtype, eng.device, n_slots, eng.max_seq,
+                         pool_tokens=pool_tokens, block=block, scratch_slot=scratch)
         # MXLLM_DECODE_COMBINE=fused: the split-K partials merge inside the attention launch (the
         # last workgroup of each (seq, kv-head) combines; these counters stay zero between calls)
         # instead of the combine kernel -- measured slower in the graphed step at every batch
@@ -66,7 +74,8 @@ class LlamaSteps:
         return kv
 
     def cached_bytes(self, n: int) -> int:
-        return n * sum(c.shape[1] * c.shape[3] * c.element_size() for c in self.eng.kv.k + self.eng.kv.v)
+        exps = 1 / kv8.GROUP if self.kv8 else 0
+        return int(n * sum(c.shape[1] * (c.shape[3] * c.element_size() + exps) for c in self.eng.kv.k + self.eng.kv.v))
 
     def hidden(self, ids: list[int]) -> torch.Tensor:
         return self.model.hidden_states(torch.tensor([ids], dtype=torch.long, device=self.eng.device))
@@ -81,12 +90,17 @@ class LlamaSteps:
         for S in lens:
             offs.append(offs[-1] + S)
 
-        rows = None
+        rows = runs = None
         if ops.use_native(x):
             rows = PromptRows(lens, eng.device, slots)
             blocks, longest = rows.attn_blocks(max(lens)), max(lens)
+        if self.kv8:
+            runs = kv8.prompt_runs([0] * len(lens), lens, slots, eng.device)
 
         def attn(i, qkv):
+            if runs is not None:
+                q, k, v = kv8.append_prompts(qkv, m.rope_cos, m.rope_sin, runs, eng.kv.pages(i), c.n_heads)
+                return kv8.prompt_attention(q, k, v, lens, blocks if rows is not None else None)
             if rows is not None:
                 return ops.native().prompt_attention(qkv.contiguous(), m.rope_cos, m.rope_sin, rows.rowinfo, blocks, longest,
                                                      c.n_heads, c.n_kv_heads, eng.kv.k[i], eng.kv.v[i], eng.kv.bt,
@@ -219,6 +233,10 @@ class LlamaSteps:
                                                              1.0 / math.sqrt(c.head_dim), 1, bt)
                 return ops.native().decode_attn(q, self.eng.kv.k[i], self.eng.kv.v[i], pos, sl, max_len,
                                                 1.0 / math.sqrt(c.head_dim), 1, bt, cnt)
+            if self.kv8:
+                pages = self.eng.kv.pages(i)
+                q = kv8.append_tokens(qkv, m.rope_cos, m.rope_sin, pos, sl, pages, c.n_heads)
+                return kv8.decode_attention(q, pages, pos, sl, max_len)
             return dops.decode_attention(qkv, m.rope_cos, m.rope_sin, self.eng.kv.k[i], self.eng.kv.v[i], pos, sl,
                                          c.n_heads, c.n_kv_heads, c.head_dim, max_len, bt, cnt)
 
@@ -226,7 +244,7 @@ class LlamaSteps:
             # QKV GEMM with the RoPE/cache-append epilogue; a few rows also with the RMSNorm prologue
             # (one launch), more rows after the RMSNorm kernel
             w, scale = self._stream_weight(layer.wqkv, B)
-            if not (_ROPE_FUSED and self.eng.tp is None and w is not None):
+            if not (_ROPE_FUSED and self.eng.tp is None and w is not None) or self.kv8:
                 return None
             rope = (w, m.rope_cos, m.rope_sin, pos, sl, self.eng.kv.k[i], self.eng.kv.v[i],
                     c.n_heads, c.n_kv_heads, bt, scale)
@@ -251,6 +269,8 @@ class RowSteps:
     def __init__(self, eng):
         if eng.tp is not None:
             raise NotImplementedError(f"{type(eng.model).__name__} is served on one GPU (no tensor-parallel sharding)")
+        if eng.kv_dtype != "bf16":
+            raise ValueError(f"kv_dtype {eng.kv_dtype}: {type(eng.model).__name__} keeps its caches in the model's type")
         self.eng, self.model, self.cfg = weakref.proxy(eng), eng.model, eng.cfg  # no cycle: caches go with the engine
 
     def _ids(self, prompts: list[list[int]]) -> torch.Tensor:
