@@ -102,39 +102,50 @@ __device__ __forceinline__ double lane_sum(double v) {
   const uint64_t other = ((uint64_t)lane_dpp<C>((uint32_t)(b >> 32)) << 32) | lane_dpp<C>((uint32_t)b);
   return v + __builtin_bit_cast(double, other);
 }
-// n = x r w (w null: x), turned by the angles of cos, sin; T: float or double
+// a, b: the pairs' halves; n = x r w (w null: x), turned by the angles of cos, sin; T: float or double.  Eight pairs at a time: 16
+// in flight in 64 bits take 244 registers, two waves a SIMD (a prompt of 4096 rows of 48 heads of 128 31.6 us, so 29.3; four
+// waves a SIMD, with registers in memory, 40).
 template <typename T, int P>
 __device__ __forceinline__ void norm_turn(float (&a)[P], float (&b)[P], const uint16_t* w, int half, const float* cosb,
                                           const float* sinb, T eps) {
-  T x[P], y[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) x[j] = a[j], y[j] = b[j];
+  constexpr int N = P < 8 ? P : 8;
+  T r = 1;
   if (w) {
     T ss = 0;
-    float w1[P], w2[P];
-    load_bf<P>(w, w1);
-    load_bf<P>(w + half, w2);
 #pragma unroll
-    for (int j = 0; j < P; ++j) ss += x[j] * x[j] + y[j] * y[j];
+    for (int j = 0; j < P; ++j) ss += (T)a[j] * (T)a[j] + (T)b[j] * (T)b[j];
     ss = lane_sum<2>(lane_sum<1>(ss)) * (T)(1.0 / (2 * half)) + eps;
-    T r;
     if constexpr (sizeof(T) == 8) r = 1.0 / sqrt(ss);
     else r = rsqrtf(ss);
+    if constexpr (sizeof(T) == 8) {  // (made 64 bits anew below: kept, they are 4 P registers)
 #pragma unroll
-    for (int j = 0; j < P; ++j) x[j] = x[j] * r * (T)w1[j], y[j] = y[j] * r * (T)w2[j];
-  }
-  float cs[P], sn[P];
-  load_f32<P>(cosb, cs);
-  load_f32<P>(sinb, sn);
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    if constexpr (sizeof(T) == 8) {
-      a[j] = odd_f32(x[j] * (T)cs[j] - y[j] * (T)sn[j]);
-      b[j] = odd_f32(y[j] * (T)cs[j] + x[j] * (T)sn[j]);
-    } else {
-      a[j] = rope_lo(x[j], y[j], cs[j], sn[j]);
-      b[j] = rope_hi(x[j], y[j], cs[j], sn[j]);
+      for (int j = 0; j < P; ++j) asm volatile("" : "+v"(a[j]), "+v"(b[j]));
     }
+  }
+#pragma unroll
+  for (int p = 0; p < P; p += N) {
+    float cs[N], sn[N], w1[N], w2[N];
+    load_f32<N>(cosb + p, cs);
+    load_f32<N>(sinb + p, sn);
+    if (w) {
+      load_bf<N>(w + p, w1);
+      load_bf<N>(w + half + p, w2);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) w1[j] = w2[j] = 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const T x = (T)a[p + j] * r * (T)w1[j], y = (T)b[p + j] * r * (T)w2[j], c = cs[j], s = sn[j];
+      if constexpr (sizeof(T) == 8) {
+        a[p + j] = odd_f32(x * c - y * s);
+        b[p + j] = odd_f32(y * c + x * s);
+      } else {
+        a[p + j] = rope_lo(x, y, c, s);
+        b[p + j] = rope_hi(x, y, c, s);
+      }
+    }
+    if (sizeof(T) == 8 && P > N) __builtin_amdgcn_sched_barrier(0);
   }
 }
 // |x| where it is a number
@@ -155,11 +166,36 @@ __global__ void __launch_bounds__(256)
                       uint16_t* __restrict__ vout, Kv8Pages pg, int Hq) {
   constexpr int P = D / 8, HALF = D / 2;
   const int Hkv = pg.Hkv, NH = Hq + 2 * Hkv;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= (int64_t)n * NH) return;
-  const int at = (int)(item / NH), head = (int)(item % NH);
+  int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, row = lane >> 2, c = P * (lane & 3);
   const int cap = (int)min((int64_t)pg.maxp * pg.block, (int64_t)turns);  // positions that a sequence can have
+  if constexpr (!RUNS) {
+    // single tokens: the first waves have 16 query heads each, of whatever rows, the others a key or value head of a row
+    const int64_t heads = (int64_t)n * Hq, first = (heads + kUnit - 1) / kUnit;
+    if (item < first) {
+      const int64_t h = min(item * kUnit + row, heads - 1);  // (lanes past the end help with the sums of a norm)
+      const int at = (int)(h / Hq), head = (int)(h % Hq), p = index[at], s = slots ? slots[at] : at;
+      const bool place = (unsigned)p < (unsigned)cap && (unsigned)s < (unsigned)pg.slots;  // else its queries are zero
+      const uint16_t* src = qkv + at * ld + head * D + c;
+      float a[P], b[P];
+      load_bf<P>(src, a);
+      load_bf<P>(src + HALF, b);
+      const int64_t turn = (int64_t)(place ? p : 0) * HALF + c;
+      norm_turn<float, P>(a, b, wq ? wq + c : nullptr, HALF, cosb + turn, sinb + turn, (float)eps);
+#pragma unroll
+      for (int j = 0; j < P; ++j) a[j] = place ? a[j] : 0.f, b[j] = place ? b[j] : 0.f;
+      if (item * kUnit + row < heads) {
+        uint16_t* dst = q + h * D + c;
+        store_bf<P>(dst, a);
+        store_bf<P>(dst + HALF, b);
+      }
+      return;
+    }
+    item -= first;
+  }
+  const int H = RUNS ? NH : 2 * Hkv;  // heads of a row here
+  if (item >= (int64_t)n * H) return;
+  const int at = (int)(item / H), head = (int)(item % H) + (RUNS ? 0 : Hq);
   int p0, slot, tk = -1;  // tk: the row of qkv of this lane's position, -1: none
   if constexpr (RUNS) {
     const int4 r = reinterpret_cast<const int4*>(index)[at];
@@ -171,35 +207,24 @@ __global__ void __launch_bounds__(256)
     if (i >= 0 && i < r.y) tk = r.x + i;
   } else {
     p0 = index[at], slot = slots ? slots[at] : at;
-    if ((unsigned)p0 >= (unsigned)cap || (unsigned)slot >= (unsigned)pg.slots) {  // no place: its queries are zero
-      if (head < Hq && row == 0) {
-        const float zero[P] = {};
-        store_bf<P>(q + ((int64_t)at * Hq + head) * D + c, zero);
-        store_bf<P>(q + ((int64_t)at * Hq + head) * D + HALF + c, zero);
-      }
-      return;
-    }
-    if (head < Hq) {
-      if (row == p0 % kUnit) tk = at;
-    } else {
-      // rows of the same group in this call belong to the first of them (of the same position the last one stays)
-      bool found = false;
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        const int p = i < n ? index[i] : -1, s = i < n ? (slots ? slots[i] : i) : -1;
-        uint64_t same = __ballot(s == slot && p >= 0 && p / kUnit == p0 / kUnit && p < cap);
-        if (!same) continue;
-        if (!found && i0 + __ffsll((unsigned long long)same) - 1 != at) return;
-        found = true;
-        for (; same; same &= same - 1) {
-          const int l = __ffsll((unsigned long long)same) - 1;
-          if (row == __builtin_amdgcn_readlane(p, l) % kUnit) tk = i0 + l;
-        }
+    if ((unsigned)p0 >= (unsigned)cap || (unsigned)slot >= (unsigned)pg.slots) return;
+    // rows of the same group in this call belong to the first of them (of the same position the last one stays)
+    bool found = false;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      const int i = i0 + lane;
+      const int p = i < n ? index[i] : -1, s = i < n ? (slots ? slots[i] : i) : -1;
+      uint64_t same = __ballot(s == slot && p >= 0 && p / kUnit == p0 / kUnit && p < cap);
+      if (!same) continue;
+      if (!found && i0 + __ffsll((unsigned long long)same) - 1 != at) return;
+      found = true;
+      for (; same; same &= same - 1) {
+        const int l = __ffsll((unsigned long long)same) - 1;
+        if (row == __builtin_amdgcn_readlane(p, l) % kUnit) tk = i0 + l;
       }
     }
   }
   const int group = p0 / kUnit;
-  const bool isq = head < Hq, isv = head >= Hq + Hkv, on = tk >= 0;
+  const bool isq = RUNS && head < Hq, isv = head >= Hq + Hkv, on = tk >= 0;
   float a[P], b[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) a[j] = b[j] = 0.f;
@@ -222,18 +247,11 @@ __global__ void __launch_bounds__(256)
     if (isq) norm_turn<float, P>(a, b, wq ? wq + c : nullptr, HALF, cosb + turn, sinb + turn, (float)eps);
     else norm_turn<double, P>(a, b, wk ? wk + c : nullptr, HALF, cosb + turn, sinb + turn, eps);
   }
-  if (isq || RUNS) {
-    uint16_t* dst;
-    if constexpr (RUNS) {
-      dst = isq ? q + ((int64_t)head * T + tk) * D
-                : (isv ? vout : kout) + ((int64_t)(head - (isv ? Hq + Hkv : Hq)) * T + tk) * D;
-    } else {
-      dst = q + ((int64_t)tk * Hq + head) * D;
-    }
-    if (on) {
-      store_bf<P>(dst + c, a);
-      store_bf<P>(dst + HALF + c, b);
-    }
+  if (RUNS && on) {
+    uint16_t* dst = isq ? q + ((int64_t)head * T + tk) * D
+                        : (isv ? vout : kout) + ((int64_t)(head - (isv ? Hq + Hkv : Hq)) * T + tk) * D;
+    store_bf<P>(dst + c, a);
+    store_bf<P>(dst + HALF + c, b);
   }
   if (isq || unit < 0) return;
   float top = 0.f;
@@ -308,7 +326,9 @@ extern "C" int mx_kv8_append(const uint16_t* qkv, int64_t ld, const float* cosb,
                              const uint16_t* wk, double eps, uint16_t* q, uint16_t* kout, uint16_t* vout, const Kv8Pages* cache,
                              int Hq, int D, hipStream_t stream) {
   if (n <= 0) return 0;
-  const int64_t blocks = ((int64_t)n * (Hq + 2 * cache->Hkv) + 3) / 4;
+  const int64_t waves = runs ? (int64_t)n * (Hq + 2 * cache->Hkv)
+                             : ((int64_t)n * Hq + kUnit - 1) / kUnit + (int64_t)n * 2 * cache->Hkv;
+  const int64_t blocks = (waves + 3) / 4;
   if (blocks > INT32_MAX) return -1;
 #define APPEND(DD, RR)                                                                                                \
   kv8_append_kernel<DD, RR><<<(unsigned)blocks, 256, 0, stream>>>(qkv, ld, cosb, sinb, turns, index, slots, n, T, wq, \
