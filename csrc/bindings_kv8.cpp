@@ -3,6 +3,9 @@
 #include "bindings_util.h"
 #include "kernels/kv8_pages.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
@@ -107,6 +110,57 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor
   MX_CHECK(rc != -1, "qk_norm_rope_bwd: too many rows");
   MX_OK(rc);
   return {dqkv, dwq, dwk};
+}
+
+// The same for autograd, here as its Python form (mxllm/ops/attention.py, which a weight with an owner takes) costs 40 us of the host's
+// time a step more, as much as 2,048 rows of 48 heads of 128 take forward and backward.
+struct QKNormRope : torch::autograd::Function<QKNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv,
+                                                const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& cos,
+                                                const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                                double eps, const OptTensor& positions) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [q, k, v] = qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
+    ctx->save_for_backward({qkv, wq, wk, cos, sin, given(positions) ? *positions : at::Tensor()});
+    ctx->saved_data["Hkv"] = Hkv;
+    ctx->saved_data["eps"] = eps;
+    return {q, k, v};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& g) {
+    const auto saved = ctx->get_saved_variables();
+    const bool need_q = ctx->needs_input_grad(1), need_k = ctx->needs_input_grad(2);
+    torch::autograd::variable_list out(12);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dqkv, dwq, dwk] = qk_norm_rope_bwd(g[0].contiguous(), g[1].contiguous(), g[2].contiguous(), saved[0], saved[1],
+                                               saved[2], saved[3], saved[4], ctx->saved_data["Hkv"].toInt(),
+                                               ctx->saved_data["eps"].toDouble(),
+                                               saved[5].defined() ? OptTensor(saved[5]) : c10::nullopt, 0, need_q || need_k, false);
+      out[0] = dqkv;
+      if (need_q) out[1] = dwq;
+      if (need_k) out[2] = dwk;
+    }
+    if (at::GradMode::is_enabled()) {  // its own gradient is not known: whoever asks for it is told
+      torch::autograd::variable_list in;
+      for (int i = 0; i < 3; ++i)
+        if (out[i].defined()) in.push_back(out[i].detach().requires_grad_());
+      const auto told = (*std::make_shared<torch::autograd::DelayedError>("qk_norm_rope is differentiable once",
+                                                                          (int64_t)in.size()))(std::move(in));
+      for (int i = 0, j = 0; i < 3; ++i)
+        if (out[i].defined()) out[i] = told[j++];
+    }
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_grad(const at::Tensor& qkv, const at::Tensor& wq,
+                                                                 const at::Tensor& wk, const at::Tensor& cos,
+                                                                 const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq,
+                                                                 int64_t Hkv, int64_t D, double eps, const OptTensor& positions) {
+  const auto out = QKNormRope::apply(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
+  return {out[0], out[1], out[2]};
 }
 
 // ---------------------------------------------------------------- the cache in 8 bits
@@ -279,3 +333,5 @@ TORCH_LIBRARY_IMPL(mxllm, CUDA, m) {
   m.impl("kv8_read", &kv8_read);
   m.impl("kv8_decode_attn", &kv8_decode_attn);
 }
+
+TORCH_LIBRARY_IMPL(mxllm, AutogradCUDA, m) { m.impl("qk_norm_rope", &qk_norm_rope_grad); }

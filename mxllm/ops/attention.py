@@ -132,12 +132,16 @@ def dq_mode() -> int:
     return m
 
 
+def _owned(w: torch.Tensor) -> bool:
+    """Whether a trainer keeps ``w``'s gradient (mxllm/parallel/grad_ready.py)."""
+    return w.is_leaf and any(hasattr(w, a) for a in ("_mx_grad32", "_mx_grad_fresh", "_mx_on_grad_ready"))
+
+
 def _norm_grads(ctx, dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad):
     """(d(qkv), dw_q, dw_k for autograd) of ``qk_norm_rope``: a weight with an owner that keeps its gradient (a trainer)
     takes it from the f32 sums with one rounding, None for autograd then."""
     need = ctx.needs_input_grad[1:3]
-    owned = [n and any(hasattr(w, a) for a in ("_mx_grad32", "_mx_grad_fresh", "_mx_on_grad_ready"))
-             for n, w in zip(need, ctx.leaves)]
+    owned = [n and w is not None and _owned(w) for n, w in zip(need, ctx.leaves)]
     dqkv, *dws = native().qk_norm_rope_bwd(dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad, any(need),
                                            any(owned))
     out = [None, None]
@@ -148,6 +152,8 @@ def _norm_grads(ctx, dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, gra
 
 
 class _QKNormRopeFn(torch.autograd.Function):
+    """``qk_norm_rope`` where a weight's gradient has an owner; else the op's own autograd (csrc/bindings_kv8.cpp)."""
+
     @staticmethod
     def forward(ctx, qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions):
         q, k, v = native().qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions)
@@ -197,7 +203,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     the table ``cos``, ``sin`` [positions, D / 2] comes out as NaN.  Differentiable once, in qkv and both weights
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
-        return _QKNormRopeFn.apply(rows_view(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+        run = _QKNormRopeFn.apply if _owned(q_norm) or _owned(k_norm) else native().qk_norm_rope
+        return run(rows_view(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
     return ref.qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
 
 
