@@ -91,6 +91,12 @@ def untransformed(*ts: torch.Tensor | None) -> bool:
                 or torch._C._functorch.maybe_current_level() is not None or torch._C._get_tracing_state() is not None)
 
 
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """:func:`rows_view` whose rows also start at multiples of 16 bytes."""
+    t = rows_view(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def rows_view(t: torch.Tensor) -> torch.Tensor:
     """``t`` if it is a 2-D row-strided view the kernels accept (unit inner
     stride, row stride a multiple of 8: e.g. the left part of a padded

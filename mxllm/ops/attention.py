@@ -25,7 +25,7 @@ from torch.autograd.function import once_differentiable
 
 from . import reference as ref
 from ..parallel.grad_ready import accum_grad
-from ._ext import native, rows_view, use_native
+from ._ext import native, rows16, use_native
 
 
 def split_heads_ref(qkv: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, D: int):
@@ -204,7 +204,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
         run = _QKNormRopeFn.apply if _owned(q_norm) or _owned(k_norm) else native().qk_norm_rope
-        return run(rows_view(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+        return run(rows16(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
     return ref.qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
 
 
@@ -218,7 +218,7 @@ def attention_block(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, B: 
     if norms is not None:
         wq, wk, eps = norms
         if use_native(qkv):
-            return _NormAttnBlockFn.apply(rows_view(qkv), wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad)
+            return _NormAttnBlockFn.apply(rows16(qkv), wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad)
         q, k, v = ref.qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps)
         return ref.attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal=causal).reshape(B * S, Hq * D)
     if use_native(qkv):

@@ -21,7 +21,7 @@ from typing import NamedTuple
 import torch
 
 from . import reference as ref
-from ._ext import native, rows_view, use_native
+from ._ext import native, rows16, use_native
 
 GROUP = 16  # positions that share an exponent
 E4M3 = torch.float8_e4m3fn
@@ -96,7 +96,7 @@ def append_tokens(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: 
     the queries [B, Hq, D].  Rows may share a sequence, and a position (the last row then stays).  A row without a place
     (a negative position or slot, or one past the block table or the rotation table) is not kept, and its query is zero."""
     if use_native(qkv):
-        return native().kv8_append_tokens(rows_view(qkv), cos, sin, pos, slots, *pages, Hq, q_norm, k_norm, eps)
+        return native().kv8_append_tokens(rows16(qkv), cos, sin, pos, slots, *pages, Hq, q_norm, k_norm, eps)
     T, Hkv, D = _check_rows(qkv, cos, sin, pages, Hq, q_norm, k_norm)
     _check_ints(pos, (T,), "pos")
     where = _slots(slots, T)
@@ -109,7 +109,7 @@ def append_tokens(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: 
             groups.setdefault((s, p // GROUP), {})[p % GROUP] = t
     for (s, g), rows in groups.items():
         _store(pages, s, g, rows, k, v)
-    q[~torch.tensor(ok, dtype=torch.bool)] = 0
+    q[~torch.tensor(ok, dtype=torch.bool, device=q.device)] = 0
     return q.to(qkv.dtype)
 
 
@@ -120,15 +120,15 @@ def append_prompts(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, runs
     q [Hq, T, D] and k, v [Hkv, T, D], normed and rotated but not rounded to 8 bits, for the attention of the prompt.  A run
     without a place is left out, its rows' outputs with it."""
     if use_native(qkv):
-        return native().kv8_append_prompts(rows_view(qkv), cos, sin, runs, *pages, Hq, q_norm, k_norm, eps)
+        return native().kv8_append_prompts(rows16(qkv), cos, sin, runs, *pages, Hq, q_norm, k_norm, eps)
     T, Hkv, D = _check_rows(qkv, cos, sin, pages, Hq, q_norm, k_norm)
     _check_ints(runs, (runs.shape[0] if runs.dim() else -1, 4), "runs")
     cap = min(pages.table.shape[1] * pages.k.shape[2], cos.shape[0])
     table = [r for r in runs.tolist() if r[0] >= 0 and 1 <= r[1] <= GROUP and r[0] + r[1] <= T and r[3] >= 0 and
              r[3] + r[1] <= cap and r[3] % GROUP + r[1] <= GROUP and 0 <= r[2] < pages.table.shape[0]]
-    pos = torch.zeros(T, dtype=torch.long)
+    pos = torch.zeros(T, dtype=torch.long, device=qkv.device)
     for t0, n, _, p0 in table:
-        pos[t0:t0 + n] = torch.arange(p0, p0 + n)
+        pos[t0:t0 + n] = torch.arange(p0, p0 + n, device=qkv.device)
     q, k, v = _heads(qkv, cos, sin, pos, Hq, Hkv, D, q_norm, k_norm, eps)
     for t0, n, s, p0 in table:
         _store(pages, s, p0 // GROUP, {p0 % GROUP + i: t0 + i for i in range(n)}, k, v)
@@ -160,7 +160,7 @@ def read(pages: Pages, slots: torch.Tensor | None, starts: torch.Tensor, ends: t
     _check_ints(ends, (B,), "ends")
     _check_pages(pages)
     where = _slots(slots, B)
-    out = [torch.zeros(B, pages.k.shape[1], n, pages.k.shape[3], dtype=torch.bfloat16) for _ in range(2)]
+    out = [torch.zeros(B, pages.k.shape[1], n, pages.k.shape[3], dtype=torch.bfloat16, device=pages.k.device) for _ in range(2)]
     for b, (s, a, e) in enumerate(zip(where, starts.tolist(), ends.tolist())):
         lo, hi = max(a, 0), min(a + n, e, pages.table.shape[1] * pages.k.shape[2])
         if 0 <= s < pages.table.shape[0] and lo < hi:
@@ -184,7 +184,7 @@ def decode_attention(q: torch.Tensor, pages: Pages, pos: torch.Tensor, slots: to
         raise ValueError(f"q {tuple(q.shape)} over a cache of {Hkv} heads of {pages.k.shape[3]}, max_len {max_len}, scale {scale}")
     _check_ints(pos, (B,), "pos")
     cap = min(max_len, pages.table.shape[1] * pages.k.shape[2])
-    out = torch.zeros(B, Hq, D)
+    out = torch.zeros(B, Hq, D, device=q.device)
     for b, (p, s) in enumerate(zip(pos.tolist(), _slots(slots, B))):
         n = min(p + 1, cap)
         if n > 0 and 0 <= s < pages.table.shape[0]:
@@ -262,8 +262,8 @@ def _store(pages: Pages, slot: int, group: int, rows: dict[int, int], k: torch.T
     if not 0 <= page < pages.k.shape[0]:
         return
     at = group * GROUP % block
-    new, src = torch.tensor(sorted(rows)), torch.tensor([rows[r] for r in sorted(rows)])
-    held = torch.tensor([r for r in range(max(rows)) if r not in rows], dtype=torch.long)
+    new, src, held = (torch.tensor(r, dtype=torch.long, device=k.device) for r in (
+        sorted(rows), [rows[r] for r in sorted(rows)], [r for r in range(max(rows)) if r not in rows]))
     for x, codes, exps in ((k, pages.k, pages.k_exp), (v, pages.v, pages.v_exp)):
         x = x[src].transpose(0, 1)  # [Hkv, rows, D]
         e = exponents(torch.where(torch.isfinite(x), x.abs(), 0.0).amax((1, 2)))
@@ -279,7 +279,7 @@ def _store(pages: Pages, slot: int, group: int, rows: dict[int, int], k: torch.T
 
 def _rows(pages: Pages, slot: int, lo: int, hi: int):
     """f32 [Hkv, hi - lo, D] of keys and values of positions lo .. hi - 1; NaN where the table names no page of the pool."""
-    p = torch.arange(lo, hi)
+    p = torch.arange(lo, hi, device=pages.k.device)
     block = pages.k.shape[2]
     page = pages.table[slot][p // block].long()
     ok = (page >= 0) & (page < pages.k.shape[0])

@@ -61,7 +61,9 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     rotated at its row's position; f32 in between, one rounding."""
     x = qkv.view(B, S, Hq + 2 * Hkv, D)
     pos = torch.arange(S, device=qkv.device).expand(B, S) if positions is None else positions.view(B, S).long()
-    c, s = cos[pos][:, :, None].float(), sin[pos][:, :, None].float()
+    there = ((pos >= 0) & (pos < cos.shape[0]))[:, :, None, None]
+    pos = pos.clamp(0, cos.shape[0] - 1)
+    c, s = (torch.where(there, t[pos][:, :, None].float(), float("nan")) for t in (cos, sin))
 
     def one(h, w):
         h = h.float()

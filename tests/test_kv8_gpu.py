@@ -336,6 +336,25 @@ def test_prompt_then_tokens_is_attention_over_all(gpu):
         assert torch.equal(o, kv8.decode_attention(qi, p, _i32([i], gpu), _i32([1], gpu), i + 1)) or i + 1 > 512
 
 
+def test_the_plain_forms_on_the_gpu_are_those_on_the_cpu(gpu, monkeypatch):
+    """MXLLM_REFERENCE_OPS=1, which turns the kernels off."""
+    D, Hq, Hkv = 32, 4, 2
+    cos, sin = (t.to(gpu) for t in _tables(60, D))
+    qkv = _rows(50, Hq, Hkv, D).to(gpu)
+    out = []
+    for plain in (False, True):
+        if plain:
+            monkeypatch.setenv("MXLLM_REFERENCE_OPS", "1")
+        p = _to(_pages(2, 4, 9, Hkv, 16, D, fill=False), gpu)  # (positions 0 .. 2 hold zeros)
+        q, k, v = kv8.append_prompts(qkv[:49], cos, sin, kv8.prompt_runs([3], [49], [1], gpu), p, Hq)
+        q1 = kv8.append_tokens(qkv[49:], cos, sin, _i32([52], gpu), _i32([1], gpu), p, Hq)
+        o = kv8.decode_attention(q1, p, _i32([52], gpu), _i32([1], gpu), 64)
+        out.append((p, k, v, *kv8.read(p, _i32([1], gpu), _i32([3], gpu), _i32([53], gpu), 50), o))
+    a, b = out
+    assert _same(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[1:5], b[1:5]))
+    assert float((a[5].double() - b[5].double()).norm() / b[5].double().norm()) < 2 * HALF
+
+
 def test_refusals(gpu):
     Hq, Hkv, D = 4, 2, 64
     cos, sin = (t.to(gpu) for t in _tables(40, D))

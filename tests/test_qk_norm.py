@@ -150,6 +150,34 @@ def test_unused_outputs_and_frozen_weights(gpu):
         g.sum().backward()
 
 
+def _outside(dev):
+    Hq, Hkv, D = 4, 2, 64
+    (qkv, wq, wk, *_), cos, sin = _inputs(dev, 1, 4, Hq, Hkv, D)
+    pos = torch.tensor([0, -1, 3, 4], dtype=torch.int32, device=dev)
+    q, k, v = ops.qk_norm_rope(qkv, wq, wk, cos, sin, 1, 4, Hq, Hkv, D, EPS, pos)
+    bad = torch.isnan(q[0, :, :, 0]).all(0).tolist()
+    assert bad == [False, True, False, True] and torch.isnan(k[0, :, 1]).all() and not torch.isnan(v).any()
+
+
+def test_positions_outside_the_table_plain():
+    _outside("cpu")
+
+
+@pytest.mark.gpu
+def test_one_weight_for_both_norms_and_rows_at_odd_places(gpu):
+    """A weight that is both norms' has the sum of their gradients; rows that start between pieces of 16 bytes are copied."""
+    B, S, Hq, Hkv, D = 1, 9, 4, 2, 64
+    (qkv, w, _, gq, gk, gv), cos, sin = _inputs(gpu, B, S, Hq, Hkv, D)
+    p, a, b = (w.clone().requires_grad_() for _ in range(3))
+    one = torch.autograd.grad(ops.qk_norm_rope(qkv, p, p, cos, sin, B, S, Hq, Hkv, D), p, (gq, gk, gv))[0]
+    two = torch.autograd.grad(ops.qk_norm_rope(qkv, a, b, cos, sin, B, S, Hq, Hkv, D), (a, b), (gq, gk, gv))
+    assert torch.equal(one, two[0] + two[1])
+    wide = torch.zeros(S, qkv.shape[1] + 8, device=gpu, dtype=torch.bfloat16)
+    wide[:, 3:3 + qkv.shape[1]] = qkv
+    out = ops.qk_norm_rope(wide[:, 3:3 + qkv.shape[1]], w, w, cos, sin, B, S, Hq, Hkv, D)
+    assert all(torch.equal(x, y) for x, y in zip(out, ops.qk_norm_rope(qkv, w, w, cos, sin, B, S, Hq, Hkv, D)))
+
+
 @pytest.mark.gpu
 def test_no_rows_and_positions_outside_the_table(gpu):
     Hq, Hkv, D = 4, 2, 64
@@ -158,11 +186,7 @@ def test_no_rows_and_positions_outside_the_table(gpu):
     out = ops.qk_norm_rope(*leaves, cos, sin, 0, 5, Hq, Hkv, D, EPS, torch.zeros(0, dtype=torch.int32, device=gpu))
     grads = torch.autograd.grad(out, leaves, [torch.zeros_like(o) for o in out])
     assert out[0].shape == (0, Hq, 5, D) and not grads[1].any() and not grads[2].any()
-    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, 1, 4, Hq, Hkv, D)
-    pos = torch.tensor([0, -1, 3, 4], dtype=torch.int32, device=gpu)
-    q, k, v = ops.qk_norm_rope(qkv, wq, wk, cos, sin, 1, 4, Hq, Hkv, D, EPS, pos)
-    bad = torch.isnan(q[0, :, :, 0]).all(0).tolist()
-    assert bad == [False, True, False, True] and torch.isnan(k[0, :, 1]).all() and not torch.isnan(v).any()
+    _outside(gpu)
 
 
 @pytest.mark.gpu
@@ -214,7 +238,7 @@ def test_attention_block_with_norms(gpu, D, Hq, Hkv, S):
     wg = torch.autograd.grad(want, exact, do.double().cpu())
 
     def rel(a, b):
-        return float((a.double().cpu() - b).norm() / b.norm())
+        return float((a.detach().double().cpu() - b.detach()).norm() / b.detach().norm())
 
     assert rel(o, want) < 2 * HALF
     assert all(rel(a, b) < 4 * HALF for a, b in zip(got, wg))
