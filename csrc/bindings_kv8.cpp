@@ -38,6 +38,14 @@ void check_heads(int64_t Hq, int64_t Hkv, int64_t D) {
   MX_CHECK(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= 4096, "query heads in whole groups of a key head, got ", Hq, " of ", Hkv);
 }
 
+// t if its rows are what the kernels read (16-byte pieces, row strides of such), else a copy of it; the checks say what is no rows
+at::Tensor rows16(const at::Tensor& t) {
+  if (t.dim() != 2 || (t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 &&
+                       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 int64_t check_qkv(const at::Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D) {
   const int64_t ld = check_rows_bf16(qkv, "qkv");
   MX_CHECK(qkv.size(1) == (Hq + 2 * Hkv) * D, "qkv [T, (Hq + 2 Hkv) D], got ", qkv.sizes());
@@ -47,16 +55,18 @@ int64_t check_qkv(const at::Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D) {
 
 // ---------------------------------------------------------------- norms of query and key heads, rotated
 // q [B, Hq, S, D], k, v [B, Hkv, S, D] of qkv rows [B * S, (Hq + 2 Hkv) D]
-std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& any, const at::Tensor& wq, const at::Tensor& wk,
                                                             const at::Tensor& cos, const at::Tensor& sin, int64_t B,
                                                             int64_t S, int64_t Hq, int64_t Hkv, int64_t D, double eps,
                                                             const OptTensor& positions) {
+  MX_CHECK(any.is_cuda(), "qkv must be a GPU tensor");
+  DevGuard g(any.device());
+  const at::Tensor qkv = rows16(any);
   check_heads(Hq, Hkv, D);
   const int64_t ld = check_qkv(qkv, Hq, Hkv, D);
   MX_CHECK(B >= 0 && S >= 0 && qkv.size(0) == B * S, "qkv has ", qkv.size(0), " rows, B * S = ", B * S);
   check_table(cos, sin, D, qkv);
   MX_CHECK(given(positions) || cos.size(0) >= S, "the table has ", cos.size(0), " positions, rows up to ", S);
-  DevGuard g(qkv.device());
   auto q = at::empty({B, Hq, S, D}, qkv.options()), k = at::empty({B, Hkv, S, D}, qkv.options()), v = at::empty_like(k);
   const int rc = mx_qk_norm_rope(bf(qkv), ld, check_weight(wq, D, qkv, "q_norm"), check_weight(wk, D, qkv, "k_norm"),
                                  cos.data_ptr<float>(), sin.data_ptr<float>(),
@@ -115,11 +125,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor
 // The same for autograd, here as its Python form (mxllm/ops/attention.py, which a weight with an owner takes) costs 40 us of the host's
 // time a step more, as much as 2,048 rows of 48 heads of 128 take forward and backward.
 struct QKNormRope : torch::autograd::Function<QKNormRope> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv,
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& any,
                                                 const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& cos,
                                                 const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                 double eps, const OptTensor& positions) {
     at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor qkv = rows16(any);
     auto [q, k, v] = qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
     ctx->save_for_backward({qkv, wq, wk, cos, sin, given(positions) ? *positions : at::Tensor()});
     ctx->saved_data["Hkv"] = Hkv;
@@ -191,10 +202,13 @@ mx::Kv8Pages check_pages(const at::Tensor& k, const at::Tensor& v, const at::Ten
 struct Appended {
   at::Tensor q, k, v;
 };
-Appended append(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& index,
+Appended append(const at::Tensor& qkv_any, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& index,
                 const OptTensor& slots, bool runs, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
                 const at::Tensor& ve, const at::Tensor& table, int64_t Hq, const OptTensor& wq, const OptTensor& wk,
                 double eps) {
+  MX_CHECK(qkv_any.is_cuda() && qkv_any.dim() == 2, "qkv: [T, (Hq + 2 Hkv) D] on the GPU");
+  DevGuard g(qkv_any.device());
+  const at::Tensor qkv = rows16(qkv_any);
   const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, qkv);
   const int64_t Hkv = kc.size(1), D = kc.size(3), T = qkv.size(0);
   check_heads(Hq, Hkv, D);
@@ -205,7 +219,6 @@ Appended append(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& 
   const int64_t n = runs ? index.size(0) : T;
   const int32_t* ix = runs ? check_ints(index, {n, 4}, qkv, "runs") : check_ints(index, {T}, qkv, "pos");
   const int32_t* sl = given(slots) ? check_ints(*slots, {T}, qkv, "slots") : nullptr;
-  DevGuard g(qkv.device());
   Appended out;
   if (runs) {
     out.q = at::empty({Hq, T, D}, qkv.options());
@@ -258,22 +271,24 @@ std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& kc, const at::Tens
   return {k, v};
 }
 
-at::Tensor kv8_decode_attn(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
+at::Tensor kv8_decode_attn(const at::Tensor& q_any, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
                            const at::Tensor& ve, const at::Tensor& table, const at::Tensor& pos, const OptTensor& slots,
                            int64_t max_len, double scale) {
+  MX_CHECK(q_any.is_cuda(), "q: on the GPU");
+  DevGuard g(q_any.device());
+  const bool as_is = q_any.is_contiguous() && reinterpret_cast<uintptr_t>(q_any.data_ptr()) % 16 == 0;
+  const at::Tensor q = as_is ? q_any : q_any.clone(at::MemoryFormat::Contiguous);
   check_bf16(q, "q");
   const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, q);
   MX_CHECK(q.dim() == 3 && q.size(2) == kc.size(3), "q [B, Hq, D], got ", q.sizes());
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = kc.size(1);
   check_heads(Hq, Hkv, D);
   MX_CHECK(Hq / Hkv <= 16, "up to 16 query heads a key head, got ", Hq / Hkv);
-  MX_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "q: alignment");
   MX_CHECK(max_len >= 1, "max_len: at least one position, got ", max_len);
   MX_CHECK(scale > 0 && scale <= 3.4028234663852886e38, "scale: a positive number, got ", scale);
   const int32_t* p = check_ints(pos, {B}, q, "pos");
   const int32_t* sl = given(slots) ? check_ints(*slots, {B}, q, "slots") : nullptr;
   const int64_t cap = std::min<int64_t>(max_len, (int64_t)pg.maxp * pg.block);
-  DevGuard g(q.device());
   auto out = at::empty({B, Hq * D}, q.options());
   const int64_t parts = mx_kv8_attn_parts((int)B, (int)Hkv, (int)D, (int)cap);
   at::Tensor ml, po;

@@ -21,7 +21,7 @@ from typing import NamedTuple
 import torch
 
 from . import reference as ref
-from ._ext import native, rows16, use_native
+from ._ext import native, use_native
 
 GROUP = 16  # positions that share an exponent
 E4M3 = torch.float8_e4m3fn
@@ -96,7 +96,7 @@ def append_tokens(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: 
     the queries [B, Hq, D].  Rows may share a sequence, and a position (the last row then stays).  A row without a place
     (a negative position or slot, or one past the block table or the rotation table) is not kept, and its query is zero."""
     if use_native(qkv):
-        return native().kv8_append_tokens(rows16(qkv), cos, sin, pos, slots, *pages, Hq, q_norm, k_norm, eps)
+        return native().kv8_append_tokens(qkv, cos, sin, pos, slots, *pages, Hq, q_norm, k_norm, eps)
     T, Hkv, D = _check_rows(qkv, cos, sin, pages, Hq, q_norm, k_norm)
     _check_ints(pos, (T,), "pos")
     where = _slots(slots, T)
@@ -120,7 +120,7 @@ def append_prompts(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, runs
     q [Hq, T, D] and k, v [Hkv, T, D], normed and rotated but not rounded to 8 bits, for the attention of the prompt.  A run
     without a place is left out, its rows' outputs with it."""
     if use_native(qkv):
-        return native().kv8_append_prompts(rows16(qkv), cos, sin, runs, *pages, Hq, q_norm, k_norm, eps)
+        return native().kv8_append_prompts(qkv, cos, sin, runs, *pages, Hq, q_norm, k_norm, eps)
     T, Hkv, D = _check_rows(qkv, cos, sin, pages, Hq, q_norm, k_norm)
     _check_ints(runs, (runs.shape[0] if runs.dim() else -1, 4), "runs")
     cap = min(pages.table.shape[1] * pages.k.shape[2], cos.shape[0])
@@ -176,7 +176,7 @@ def decode_attention(q: torch.Tensor, pages: Pages, pos: torch.Tensor, slots: to
     positions at it and behind are not seen), ``scale`` > 0.  A row without keys (pos < 0, or a slot that is none) gives zeros."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if use_native(q):
-        return native().kv8_decode_attn(q.contiguous(), *pages, pos, slots, max_len, scale)
+        return native().kv8_decode_attn(q, *pages, pos, slots, max_len, scale)
     _check_pages(pages)
     B, Hq, D = q.shape
     Hkv = pages.k.shape[1]
