@@ -2,7 +2,7 @@
 //   o = softmax(q k^T scale) v over positions 0 .. pos, queries of a group of heads sharing a key/value head.
 //
 // Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
-// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 55 us, where loads alone take 53 and a linear read of as much 45.
+// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 49 us, of which the merge 5; a linear read of as much takes 45.
 //
 //   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
 // by v_mfma_f32_16x16x32_bf16 on codes that become bf16 in registers, where they are exact, the units' (16 positions) powers of
@@ -11,10 +11,16 @@
 // sums of two e4m3 codes under v_mfma_scale_f32_16x16x128_f8f6f4, save 32 conversions a tile and no time, and that
 // product drops what is 2^-13 of its largest summand: outputs 2.3e-3 off in place of 2.0e-3.)
 //
-// The operands: a lane (c, g) of K has row c of a unit and the channels 64 h + 16 g .. + 15 (a dot product does not mind the
-// order, so a lane takes whole pieces of 16 bytes; queries are laid out alike), of V eight rows and D / 16 neighbouring
-// channels, whose bytes are put together row by row as the product reads them.  No tile goes through LDS.  Loads of the next
-// tile ahead of the products of the last, and more waves a CU, change nothing.
+// A wave works on tiles of two units, 32 keys and values.  They come to its own part of LDS by loads of 1 KB, whole rows, that
+// are not kept in the caches, the next tile's while this one is worked on, and nothing waits for another wave.  A lane (c, g)
+// then takes row c of each unit, pieces of 16 bytes 64 h + 16 g (a dot product does not mind the order of channels, and queries
+// are laid out alike), and of eight value rows its D / 16 channels, whose bytes are put together row by row as the product
+// reads them.  Us with what was there before, memory's caches cold / as three calls in turn leave them:
+//   a lane's rows straight to registers, kept in the caches    32 x 100 .. 2000 of 128 19.6 / 16.6, 8 x 16384 54.9 / 54.6
+//   the same, not kept (rows of half a line: 40 x 1000 .. 4000 of 64 18.2 -> 19.7)      20.6 / 20.0,            49.8 / 49.3
+//   whole rows by LDS, not kept                                                        18.2 / 17.4,            49.8 / 48.9
+//   and the next tile on its way                                                       16.8 / 15.9,            49.2 / 48.7
+// and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 67.3 cold, 6.0 TB/s; one of 700 keys does not mind.
 //
 // Rows are whole (a workgroup each, nothing to merge) or cut: the units of all sequences in a row are dealt in equal
 // shares, one a workgroup of a KV head, whose four waves share what it has of a sequence, and sequences that were cut are
@@ -26,6 +32,10 @@ namespace mx {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+constexpr int kNt = 2;  // of a load: read once
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4v& a, const u16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
@@ -42,15 +52,10 @@ struct VPiece {
 };
 template <>
 struct VPiece<8> {
-  typedef uint2 type;
+  typedef u32x2v type;
 };
-template <>
-struct VPiece<2> {
-  typedef uint16_t type;
-};
-__device__ __forceinline__ uint32_t word(uint2 v, int i) { return i ? v.y : v.x; }
+__device__ __forceinline__ uint32_t word(u32x2v v, int i) { return v[i]; }
 __device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
-__device__ __forceinline__ uint32_t word(uint16_t v, int) { return v; }
 
 // channel of k-step s of lane group g
 template <int D>
@@ -70,50 +75,84 @@ struct Kv8State {  // of one wave
     for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // two units of one wave, on their way from memory
-  struct Tile {
-    uint32_t k[2][2 * KS];          // words of the lane's channels, in the order of the k-steps
-    typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
+  // 16-byte piece `ch` of key `row` (of the tile's 32) in LDS: pieces of a row change places so that rows that start in the
+  // same bank do not meet
+  static __device__ __forceinline__ int place(int row, int ch) {
+    constexpr int N = D / 16;  // pieces of a row
+    return row * D + 16 * (ch ^ (N == 8 ? row & 7 : N == 4 ? (row >> 2) & 3 : 0));
+  }
+  // LDS addresses of a lane: of its pieces of a key (h: 64 channels further), of its channels of four value rows; units of a tile
+  // are 16 D apart, values 32 D behind keys
+  struct Places {
+    uint32_t k[D == 128 ? 2 : 1], v[4];
+
+    __device__ __forceinline__ Places(const char* lds, int c, int g) {
+      const uint32_t base = lds_addr(lds);
+      if constexpr (D == 32) k[0] = base + place(c, g >> 1) + 8 * (g & 1);
+      else {
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) k[h] = base + place(c, 4 * h + g);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = base + 32 * D + place(4 * g + i, E * c / 16) + E * c % 16;
+    }
   };
-  // k0, v0 / k1, v1: the units; ALL: every row of both is there; else lim: their last one (less than 0: none), and rows behind it
-  // are read as that row
+
+  // Two units' keys (32 rows) to LDS, then their values: k0, v0 / k1, v1: the units; ALL: every row of both is there; else lim: their
+  // last one (less than 0: none), and rows behind it are read as that row.  As the products want them, a lane a row, a load would
+  // ask for 64 pieces of as many lines; so it has whole rows, 1 KB.
   template <bool ALL>
-  static __device__ __forceinline__ void load(Tile& t, const uint8_t* __restrict__ k0, const uint8_t* __restrict__ k1,
+  static __device__ __forceinline__ void load(char* lds, const uint8_t* __restrict__ k0, const uint8_t* __restrict__ k1,
                                               const uint8_t* __restrict__ v0, const uint8_t* __restrict__ v1, int lim0,
-                                              int lim1, int c, int g) {
+                                              int lim1, int lane) {
+    constexpr int N = D / 16, ROWS = 64 / N;  // of a load
     const int z0 = max(lim0, 0), z1 = max(lim1, 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint8_t* p = (j ? k1 : k0) + (uint32_t)((ALL ? c : min(c, j ? z1 : z0)) * D + (D == 32 ? 8 : 16) * g);
-      if constexpr (D == 32) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        t.k[j][0] = w.x, t.k[j][1] = w.y;
-      } else {
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          const uint4 w = *reinterpret_cast<const uint4*>(p + 64 * h);
-          t.k[j][4 * h] = w.x, t.k[j][4 * h + 1] = w.y, t.k[j][4 * h + 2] = w.z, t.k[j][4 * h + 3] = w.w;
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const int r = ALL ? 4 * g + (s & 3) : min(4 * g + (s & 3), s < 4 ? z0 : z1);
-      t.v[s] = *reinterpret_cast<const typename VPiece<E>::type*>((s < 4 ? v0 : v1) + (uint32_t)(r * D + E * c));
+    for (int i = 0; i < 64 / ROWS; ++i) {
+      const bool val = i >= 32 / ROWS;
+      const int row = ROWS * (val ? i - 32 / ROWS : i) + lane / N, r = row & 15;
+      const bool second = ROWS == 32 ? lane >= 32 : (ROWS * i & 31) >= 16;
+      const int ch = (place(row, lane % N) - row * D) / 16;  // (the exchange is its own inverse)
+      const uint8_t* p = (val ? second ? v1 : v0 : second ? k1 : k0) + (uint32_t)((ALL ? r : min(r, second ? z1 : z0)) * D + 16 * ch);
+      __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(lds + 1024 * i), 16, 0, kNt);
     }
   }
 
   // ks: what the units' scores are multiplied by, vs: powers of two of their values
-  template <bool ALL>
-  __device__ __forceinline__ void take(const Tile& t, const u16x8 (&qf)[KS], float ks0, float ks1, float vs0, float vs1,
-                                       int lim0, int lim1, int g) {
+  template <bool ALL, int OFF>
+  __device__ __forceinline__ void take(const Places& at, const u16x8 (&qf)[KS], float ks0, float ks1, float vs0, float vs1,
+                                       int lim0, int lim1, int c, int g) {
     f32x4 sc[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        sc[j] = mfma16(__builtin_bit_cast(u32x4v, dequant8(t.k[j][2 * s], t.k[j][2 * s + 1])), qf[s], sc[j]);
+    // (one block of reads and their wait: the compiler would wait for the next tile, which is on its way to the other half)
+    if constexpr (D == 128) {
+      u32x4v w0, w1, w2, w3;
+      asm volatile("ds_read_b128 %0, %4 offset:%6\n\tds_read_b128 %1, %5 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\t"
+                   "ds_read_b128 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(w0), "=&v"(w1), "=&v"(w2), "=&v"(w3)
+                   : "v"(at.k[0]), "v"(at.k[1]), "i"(OFF), "i"(OFF + 16 * D)
+                   : "memory");
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[2], w0[3])), qf[1], sc[0]);
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[2], w2[3])), qf[1], sc[1]);
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[0], w1[1])), qf[2], sc[0]);
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[0], w3[1])), qf[2], sc[1]);
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[2], w1[3])), qf[3], sc[0]);
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[2], w3[3])), qf[3], sc[1]);
+    } else if constexpr (D == 64) {
+      u32x4v w0, w2;
+      asm volatile("ds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(w0), "=&v"(w2) : "v"(at.k[0]), "i"(OFF), "i"(OFF + 16 * D) : "memory");
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[2], w0[3])), qf[1], sc[0]);
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[2], w2[3])), qf[1], sc[1]);
+    } else {
+      u32x2v w0, w2;
+      asm volatile("ds_read_b64 %0, %2 offset:%3\n\tds_read_b64 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(w0), "=&v"(w2) : "v"(at.k[0]), "i"(OFF), "i"(OFF + 16 * D) : "memory");
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
     }
     float x[8];
 #pragma unroll
@@ -141,13 +180,25 @@ struct Kv8State {  // of one wave
       l += p;
       pb[i] = f2bf(p);
     }
+    typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
+#define KV8_READ8(OP)                                                                                                     \
+  asm volatile(OP " %0, %8 offset:%12\n\t" OP " %1, %9 offset:%12\n\t" OP " %2, %10 offset:%12\n\t" OP " %3, %11 offset:%12\n\t" \
+               OP " %4, %8 offset:%13\n\t" OP " %5, %9 offset:%13\n\t" OP " %6, %10 offset:%13\n\t" OP " %7, %11 offset:%13\n\t" \
+               "s_waitcnt lgkmcnt(0)"                                                                                      \
+               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])    \
+               : "v"(at.v[0]), "v"(at.v[1]), "v"(at.v[2]), "v"(at.v[3]), "i"(OFF), "i"(OFF + 16 * D)                       \
+               : "memory")
+    if constexpr (D == 128) KV8_READ8("ds_read_b64");
+    else if constexpr (D == 64) KV8_READ8("ds_read_b32");
+    else KV8_READ8("ds_read_u16");
+#undef KV8_READ8
     // bytes 0, 1 or 2, 3 of the words of two rows side by side, as pairs of rows of one channel each
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
       u32x4v a0, a1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w = __builtin_amdgcn_perm(word(t.v[2 * i + 1], e >> 2), word(t.v[2 * i], e >> 2),
+        const uint32_t w = __builtin_amdgcn_perm(word(v[2 * i + 1], e >> 2), word(v[2 * i], e >> 2),
                                                  e & 2 ? 0x07030602u : 0x05010400u);
         a0[i] = pair_bf16(w, i < 2 ? vs0 : vs1, false), a1[i] = pair_bf16(w, i < 2 ? vs0 : vs1, true);
       }
@@ -168,19 +219,24 @@ __device__ __forceinline__ int kv8_share(int total, int W) { return max((total +
 
 // EVEN: grid (W, Hkv), shares of all rows' units; else (Hkv, B), a workgroup a row.
 template <int D, int WAVES, bool EVEN>
-__global__ void __launch_bounds__(64 * WAVES, 3)
-    kv8_attn_kernel(const uint16_t* __restrict__ q, Kv8Pages pg, const int32_t* __restrict__ pos,
-                    const int32_t* __restrict__ slots, float* __restrict__ part_ml, float* __restrict__ part_o,
+__global__ void __launch_bounds__(64 * WAVES, 2)
+    kv8_attn_kernel(const int32_t* __restrict__ pos, const int32_t* __restrict__ slots, const int32_t* __restrict__ table,
+                    const uint16_t* __restrict__ q, uint8_t* __restrict__ keys, uint8_t* __restrict__ values,
+                    uint8_t* __restrict__ key_exps, uint8_t* __restrict__ value_exps, int nslots, int maxp, int block,
+                    int pages, int Hkv, float* __restrict__ part_ml, float* __restrict__ part_o,
                     uint16_t* __restrict__ out, int B, int Hq, int cap, int nparts, float sl) {
+  const Kv8Pages pg{keys, values, key_exps, value_exps, table, nslots, maxp, block, pages, Hkv};
   typedef Kv8State<D> State;
   constexpr int E = State::E, KS = State::KS, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
   typedef float orow_t __attribute__((ext_vector_type(E)));
-  __shared__ __attribute__((aligned(32))) float so[WAVES * 16 * ROW];
+  // of a wave: two tiles on their way, then its outputs
+  constexpr int PART = 128 * D > 64 * ROW ? 128 * D : 64 * ROW;
+  __shared__ __attribute__((aligned(32))) char smem[WAVES * PART];
   __shared__ float mls[WAVES][2][16];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4, rep = Hq / pg.Hkv;
   const int hk = EVEN ? blockIdx.y : blockIdx.x;
-  int b = EVEN ? 0 : blockIdx.y, start = 0, at = 0, end = 0, share = 1;
+  int b = EVEN ? 0 : blockIdx.y, start = 0, from_unit = 0, end = 0, share = 1;
   int i0 = 0, lens = 0, at_slot = 0;  // EVEN: lane i has row i0 + i
   const auto window = [&](int from) {
     i0 = from;
@@ -193,12 +249,12 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
     for (int f = 64 * ((B - 1) / 64); f >= 0; f -= 64) total += mine = window(f);  // (the first rows stay)
     total = __builtin_amdgcn_readfirstlane(wave_sum(total));
     share = kv8_share(total, gridDim.x);
-    at = blockIdx.x * share;
-    end = min(total, at + share);
-    if (at >= end) return;
-    while (true) {  // the row that holds unit `at`: start <= at < start + its units
+    from_unit = blockIdx.x * share;
+    end = min(total, from_unit + share);
+    if (from_unit >= end) return;
+    while (true) {  // the row that holds unit `from_unit`: start <= it < start + its units
       const int upto = (int)wave_scan((uint32_t)mine);
-      const uint64_t past = __ballot(start + upto > at);
+      const uint64_t past = __ballot(start + upto > from_unit);
       if (past) {
         const int first = __ffsll((unsigned long long)past) - 1;
         b = __builtin_amdgcn_readfirstlane(i0 + first);
@@ -221,7 +277,7 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
         continue;
       }
       from = start + kPad;  // of its keys
-      u0 = max(at - from, 0), u1 = min(end - from, n);
+      u0 = max(from_unit - from, 0), u1 = min(end - from, n);
       if (u1 <= 0) return;  // its keys begin in the next share
     } else {
       slot = slots ? slots[b] : b;
@@ -237,28 +293,53 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
     }
     State st;
     st.clear();
-    for (int v0 = u0; v0 < u1; v0 += 64) {
-      // a lane finds one unit: where it lies, and its powers of two (NaN where it lies nowhere)
-      const int m = min(64, u1 - v0);
-      const int64_t unit = kv8_unit(pg, slot, v0 + min(lane, m - 1), hk);
+    char* const kl = smem + w * PART;
+    const typename State::Places at(kl, c, g);
+    // tiles of two units, dealt to the waves in turn (side by side: 8 x WAVES KB in a row of keys, and of values); a lane finds one
+    // of the wave's next 64 units: where it lies, and its powers of two (NaN where it lies nowhere)
+    for (int t0 = u0 + 2 * w; t0 < u1; t0 += 64 * WAVES) {
+      const int mine = t0 + 2 * WAVES * (lane >> 1) + (lane & 1);
+      const int64_t unit = kv8_unit(pg, slot, min(mine, u1 - 1), hk);
       const int where = (int)max(unit, (int64_t)0);
       const float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)pg.ke[where] << 23);
       const float vs = __uint_as_float((uint32_t)pg.ve[where] << 23);
-      const auto run = [&](auto all, int j) {
-        constexpr bool ALL = decltype(all)::value;
-        const int j1 = ALL ? j + 1 : min(j + 1, m - 1), lim = len - 1 - kUnit * (v0 + j), lim1 = j1 > j ? lim - kUnit : -1;
-        const int64_t a0 = (int64_t)__builtin_amdgcn_readlane(where, j) * (kUnit * D);
-        const int64_t a1 = (int64_t)__builtin_amdgcn_readlane(where, j1) * (kUnit * D);
-        const auto of = [](float x, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
-        typename State::Tile t;
-        State::template load<ALL>(t, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, c, g);
-        __builtin_amdgcn_sched_barrier(0);  // every load is in flight before the first product waits
-        st.template take<ALL>(t, qf, of(ks, j), of(ks, j1), of(vs, j), of(vs, j1), lim, lim1, g);
+      const int tiles = min(32, (u1 - t0 + 2 * WAVES - 1) / (2 * WAVES));  // of this wave, here
+      const int whole = min(u1, len / kUnit);                                // units before this one have all their rows
+      const auto all = [&](int i) { return t0 + 2 * WAVES * i + 2 <= whole; };
+      const auto fetch = [&](int i, int half) {
+        const int64_t a0 = (int64_t)__builtin_amdgcn_readlane(where, 2 * i) * (kUnit * D);
+        const int64_t a1 = (int64_t)__builtin_amdgcn_readlane(where, 2 * i + 1) * (kUnit * D);
+        const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
+        char* to = kl + half * (64 * D);
+        if (all(i)) State::template load<true>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, 15, 15, lane);
+        else State::template load<false>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, lane);
       };
-      const int whole = min(m, max(0, len / kUnit - v0));  // units whose rows are all there
-      int j = 2 * w;  // (the waves side by side: 8 x WAVES KB in a row of keys, and of values)
-      for (; j + 2 <= whole; j += 2 * WAVES) run(std::true_type{}, j);
-      for (; j < m; j += 2 * WAVES) run(std::false_type{}, j);
+      const auto use = [&](int i, auto off) {
+        constexpr int OFF = decltype(off)::value;
+        const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
+        const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
+        if (all(i)) st.template take<true, OFF>(at, qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), 15, 15, c, g);
+        else st.template take<false, OFF>(at, qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), lim, lim1, c, g);
+      };
+      constexpr int LOADS = D / 16;  // of a tile
+      fetch(0, 0);
+      for (int i = 0; i < tiles; i += 2) {
+        if (i + 1 < tiles) {
+          fetch(i + 1, 1);
+          __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);  // the older tile has landed (only this wave reads it)
+        } else {
+          __builtin_amdgcn_s_waitcnt(0x0F70);
+        }
+        use(i, std::integral_constant<int, 0>{});
+        if (i + 1 >= tiles) break;
+        if (i + 2 < tiles) {
+          fetch(i + 2, 0);
+          __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);
+        } else {
+          __builtin_amdgcn_s_waitcnt(0x0F70);
+        }
+        use(i + 1, std::integral_constant<int, 64 * D>{});
+      }
     }
     st.l = lane_sum<32>(lane_sum<16>(st.l));
 #pragma unroll
@@ -266,7 +347,7 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
       orow_t y;
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = st.o[e][i];
-      *reinterpret_cast<orow_t*>(so + (w * 16 + c) * ROW + E * (4 * g + i)) = y;
+      *reinterpret_cast<orow_t*>(reinterpret_cast<float*>(smem + w * PART) + c * ROW + E * (4 * g + i)) = y;
     }
     if (g == 0) mls[w][0][c] = st.m, mls[w][1][c] = st.l;
     __syncthreads();
@@ -280,7 +361,7 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
       for (int x = 0; x < WAVES; ++x) {  // (a wave whose scores are NaN has no maximum, and its sum carries them)
         const float mw = mls[x][0][h], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
         L += f * mls[x][1][h];
-        acc += f * so[(x * 16 + h) * ROW + d];
+        acc += f * reinterpret_cast<const float*>(smem + x * PART)[h * ROW + d];
       }
       const int64_t bh = (int64_t)b * Hq + hk * rep + h;
       if (last == 0) {  // the row's only part is its output
@@ -291,8 +372,8 @@ __global__ void __launch_bounds__(64 * WAVES, 3)
       }
     }
     if constexpr (!EVEN) return;
-    at = start = from + n;
-    if (at >= end) return;
+    from_unit = start = from + n;
+    if (from_unit >= end) return;
     ++b;
     __syncthreads();  // the sums are read
   }
@@ -371,16 +452,16 @@ __global__ void __launch_bounds__(C* G)
 
 using namespace mx;
 
-// Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 6 us for 256 KB (43 GB/s a CU, whatever
-// its waves); cutting costs a merge and more ends, 4 to 9 us.  Us with whole rows of 4 / 8 / 16 waves, and cut:
-//   1 x 700 keys, 8 heads of 64 5.6 / 5.2 / 5.6, 7.7; of 128 8.3 / 8.0 / 8.0, 9.4; 1 x 4096 of 128 27 / 26 / 26, 11.6
-//   16 x 500 .. 2000, 8 heads of 64 12.2 / 9.6 / 9.1, 12.6;  40 x 1000 .. 4000, 5 heads of 64 22.5 / 17.1 / 15.9, 18.8
-//   32 x 100 .. 2000, 8 heads of 128 20.1 / 17.6 / 17.3, 23.6;  64 x 2048 .. 4096 77.3 / 80.9 / 85.1, 86.7
+// Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB (a CU's 60 GB/s,
+// whatever its waves); cutting costs a merge and more ends, 4 to 9 us.  Us with whole rows of 4 / 8 waves, and cut:
+//   1 x 700 keys, 8 heads of 64 5.7 / 5.1, 7.3; of 128 7.5 / 6.6, 8.7;  1 x 4096 of 128 25.6 / 18.6, 10.9
+//   16 x 500 .. 2000, 8 heads of 64 11.5 / 9.5, 13.4;  40 x 1000 .. 4000, 5 heads of 64 20.3 / 15.5, 20.4
+//   32 x 100 .. 2000, 8 heads of 128 16.6 / 16.1, 22.0;  64 x 30 .. 512 10.0 / 12.5, 18.1;  64 x 2048 .. 4096 68.9 / 70.2, 74.4
 // Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 10 us.
 static int kv8_waves(int64_t rows, int64_t cap, int D) {
   const int64_t bytes = cap * D;  // of keys
   if (bytes > (rows >= 384 ? 524288 : rows >= 128 ? 262144 : 131072)) return 0;
-  return rows >= 384 ? 4 : rows >= 96 ? 16 : 8;
+  return rows >= 384 ? 4 : 8;
 }
 // workgroups of a KV head where keys are dealt evenly: two a CU of 256
 static int kv8_shares(int Hkv) { return Hkv < 512 ? (512 + Hkv - 1) / Hkv : 1; }
@@ -408,7 +489,8 @@ struct Launch {
 template <int D, int WAVES>
 void launch_whole(const Launch& a) {
   kv8_attn_kernel<D, WAVES, false><<<dim3(a.pg.Hkv, a.B), 64 * WAVES, 0, a.stream>>>(
-      a.q, a.pg, a.pos, a.slots, nullptr, nullptr, a.out, a.B, a.Hq, a.cap, 0, a.sl);
+      a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages,
+      a.pg.Hkv, nullptr, nullptr, a.out, a.B, a.Hq, a.cap, 0, a.sl);
 }
 
 template <int D>
@@ -417,12 +499,12 @@ void launch(const Launch& a) {
   if (!nparts) {
     const int waves = kv8_waves((int64_t)a.B * Hkv, a.cap, D);
     if (waves == 4) launch_whole<D, 4>(a);
-    else if (waves == 8) launch_whole<D, 8>(a);
-    else launch_whole<D, 16>(a);
+    else launch_whole<D, 8>(a);
     return;
   }
-  kv8_attn_kernel<D, 4, true><<<dim3(W, Hkv), 256, 0, a.stream>>>(a.q, a.pg, a.pos, a.slots, a.part_ml, a.part_o, a.out,
-                                                                  a.B, a.Hq, a.cap, nparts, a.sl);
+  kv8_attn_kernel<D, 4, true><<<dim3(W, Hkv), 256, 0, a.stream>>>(
+      a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages, Hkv,
+      a.part_ml, a.part_o, a.out, a.B, a.Hq, a.cap, nparts, a.sl);
   const int rows = a.B * a.Hq;
   if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.1 -> 10.4 us, 1 x 32768 34.9 -> 19.9
     kv8_merge_kernel<D, 32, 8><<<rows * (D / 32), 256, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots, a.out, a.B,
