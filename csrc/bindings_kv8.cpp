@@ -46,6 +46,29 @@ at::Tensor rows16(const at::Tensor& t) {
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
+// t, or a copy of it at a multiple of 16 bytes
+at::Tensor placed(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 || !t.is_contiguous() ? t : t.clone();
+}
+OptTensor placed(const OptTensor& t) { return given(t) ? OptTensor(placed(*t)) : c10::nullopt; }
+
+// A backward pass takes each leaf's gradient on the stream of the leaf's accumulator, which lives as long as any graph of the leaf
+// does: captured, it would pull the default stream of a graph from before into the capture, and that ends the process.
+void check_capture(at::TensorList leaves) {
+  if (!cur_stream()) return;  // the default stream is never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  MX_OK((int)hipStreamIsCapturing(cur_stream(), &status));
+  if (status == hipStreamCaptureStatusNone) return;
+  for (const at::Tensor& t : leaves) {
+    if (!t.requires_grad() || !t.is_leaf()) continue;
+    const auto kept = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = kept ? kept->stream() : std::nullopt;
+    MX_CHECK(!stream || c10::hip::HIPStreamMasqueradingAsCUDA(*stream).stream() != nullptr,
+             "qk_norm_rope: its backward cannot be captured while another graph of the same leaf lives on the default stream; let "
+             "go of that one's outputs first, or give the captured one detached leaves");
+  }
+}
+
 int64_t check_qkv(const at::Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D) {
   const int64_t ld = check_rows_bf16(qkv, "qkv");
   MX_CHECK(qkv.size(1) == (Hq + 2 * Hkv) * D, "qkv [T, (Hq + 2 Hkv) D], got ", qkv.sizes());
@@ -55,13 +78,13 @@ int64_t check_qkv(const at::Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D) {
 
 // ---------------------------------------------------------------- norms of query and key heads, rotated
 // q [B, Hq, S, D], k, v [B, Hkv, S, D] of qkv rows [B * S, (Hq + 2 Hkv) D]
-std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& any, const at::Tensor& wq, const at::Tensor& wk,
-                                                            const at::Tensor& cos, const at::Tensor& sin, int64_t B,
-                                                            int64_t S, int64_t Hq, int64_t Hkv, int64_t D, double eps,
-                                                            const OptTensor& positions) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& any, const at::Tensor& wq_any,
+                                                            const at::Tensor& wk_any, const at::Tensor& cos_any,
+                                                            const at::Tensor& sin_any, int64_t B, int64_t S, int64_t Hq,
+                                                            int64_t Hkv, int64_t D, double eps, const OptTensor& positions) {
   MX_CHECK(any.is_cuda(), "qkv must be a GPU tensor");
   DevGuard g(any.device());
-  const at::Tensor qkv = rows16(any);
+  const at::Tensor qkv = rows16(any), wq = placed(wq_any), wk = placed(wk_any), cos = placed(cos_any), sin = placed(sin_any);
   check_heads(Hq, Hkv, D);
   const int64_t ld = check_qkv(qkv, Hq, Hkv, D);
   MX_CHECK(B >= 0 && S >= 0 && qkv.size(0) == B * S, "qkv has ", qkv.size(0), " rows, B * S = ", B * S);
@@ -79,12 +102,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& an
 }
 
 // gradients [B, H, S, D] of q, k, v, all bf16 or all f32; those of k and v as whole numbers of summands a head
-std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk,
-                                                                const at::Tensor& dv, const at::Tensor& qkv,
-                                                                const at::Tensor& wq, const at::Tensor& wk,
-                                                                const at::Tensor& cos, const at::Tensor& sin, int64_t Hkv,
-                                                                double eps, const OptTensor& positions, int64_t out_pad,
-                                                                bool need_dw, bool dw32) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq_any, const at::Tensor& dk_any,
+                                                                const at::Tensor& dv_any, const at::Tensor& any,
+                                                                const at::Tensor& wq_any, const at::Tensor& wk_any,
+                                                                const at::Tensor& cos_any, const at::Tensor& sin_any,
+                                                                int64_t Hkv, double eps, const OptTensor& positions,
+                                                                int64_t out_pad, bool need_dw, bool dw32) {
+  MX_CHECK(any.is_cuda(), "qkv must be a GPU tensor");
+  DevGuard g(any.device());
+  const at::Tensor qkv = rows16(any), wq = placed(wq_any), wk = placed(wk_any), cos = placed(cos_any), sin = placed(sin_any);
+  const at::Tensor dq = placed(dq_any), dk = placed(dk_any), dv = placed(dv_any);
   MX_CHECK(dq.dim() == 4 && dk.dim() == 4 && dv.sizes() == dk.sizes(), "gradients [B, H, S, D]");
   const int64_t B = dq.size(0), Hq = dq.size(1), S = dq.size(2), D = dq.size(3);
   check_heads(Hq, Hkv, D);
@@ -101,7 +128,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor
   MX_CHECK(out_pad >= 0 && out_pad % 8 == 0, "out_pad must be a non-negative multiple of 8");
   check_table(cos, sin, D, qkv);
   MX_CHECK(given(positions) || cos.size(0) >= S, "the table has ", cos.size(0), " positions, rows up to ", S);
-  DevGuard g(qkv.device());
   const uint16_t *pq = check_weight(wq, D, qkv, "q_norm"), *pk = check_weight(wk, D, qkv, "k_norm");
   const int64_t NHD = (Hq + 2 * Hkv) * D;
   auto dqkv = empty_rows(B * S, NHD, out_pad, qkv.options());
@@ -170,6 +196,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_grad(const at::Tenso
                                                                  const at::Tensor& wk, const at::Tensor& cos,
                                                                  const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq,
                                                                  int64_t Hkv, int64_t D, double eps, const OptTensor& positions) {
+  if (at::GradMode::is_enabled()) {
+    DevGuard g(qkv.device());
+    check_capture({qkv, wq, wk});
+  }
   const auto out = QKNormRope::apply(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
   return {out[0], out[1], out[2]};
 }
@@ -202,13 +232,15 @@ mx::Kv8Pages check_pages(const at::Tensor& k, const at::Tensor& v, const at::Ten
 struct Appended {
   at::Tensor q, k, v;
 };
-Appended append(const at::Tensor& qkv_any, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& index,
+Appended append(const at::Tensor& qkv_any, const at::Tensor& cos_any, const at::Tensor& sin_any, const at::Tensor& index_any,
                 const OptTensor& slots, bool runs, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ke,
-                const at::Tensor& ve, const at::Tensor& table, int64_t Hq, const OptTensor& wq, const OptTensor& wk,
+                const at::Tensor& ve, const at::Tensor& table, int64_t Hq, const OptTensor& wq_any, const OptTensor& wk_any,
                 double eps) {
   MX_CHECK(qkv_any.is_cuda() && qkv_any.dim() == 2, "qkv: [T, (Hq + 2 Hkv) D] on the GPU");
   DevGuard g(qkv_any.device());
-  const at::Tensor qkv = rows16(qkv_any);
+  const at::Tensor qkv = rows16(qkv_any), cos = placed(cos_any), sin = placed(sin_any);
+  const at::Tensor index = runs ? placed(index_any) : index_any;
+  const OptTensor wq = placed(wq_any), wk = placed(wk_any);
   const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, qkv);
   const int64_t Hkv = kc.size(1), D = kc.size(3), T = qkv.size(0);
   check_heads(Hq, Hkv, D);
@@ -332,6 +364,7 @@ at::Tensor prompt_rows_attention(const at::Tensor& q, const at::Tensor& k, const
 TORCH_LIBRARY_FRAGMENT(mxllm, m) {
   m.def("prompt_rows_attention(Tensor q, Tensor k, Tensor v, Tensor blocks, float scale) -> Tensor");
   m.def("qk_norm_rope(Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int B, int S, int Hq, int Hkv, int D, float eps, Tensor? positions=None) -> (Tensor, Tensor, Tensor)");
+  m.def("grads_capturable(Tensor[] leaves) -> ()");
   m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor dv, Tensor qkv, Tensor wq, Tensor wk, Tensor cos, Tensor sin, int Hkv, float eps, Tensor? positions=None, int out_pad=0, bool need_dw=True, bool dw32=False) -> (Tensor, Tensor, Tensor)");
   m.def("kv8_append_tokens(Tensor qkv, Tensor cos, Tensor sin, Tensor pos, Tensor? slots, Tensor(a!) k, Tensor(b!) v, Tensor(c!) ke, Tensor(d!) ve, Tensor table, int Hq, Tensor? wq, Tensor? wk, float eps) -> Tensor");
   m.def("kv8_append_prompts(Tensor qkv, Tensor cos, Tensor sin, Tensor runs, Tensor(a!) k, Tensor(b!) v, Tensor(c!) ke, Tensor(d!) ve, Tensor table, int Hq, Tensor? wq, Tensor? wk, float eps) -> (Tensor, Tensor, Tensor)");
@@ -342,6 +375,7 @@ TORCH_LIBRARY_FRAGMENT(mxllm, m) {
 TORCH_LIBRARY_IMPL(mxllm, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.impl("grads_capturable", &check_capture);
   m.impl("kv8_append_tokens", &kv8_append_tokens);
   m.impl("kv8_append_prompts", &kv8_append_prompts);
   m.impl("prompt_rows_attention", &prompt_rows_attention);

@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
         acc += f * reinterpret_cast<const float*>(smem + x * PART)[h * ROW + d];
       }
       const int64_t bh = (int64_t)b * Hq + hk * rep + h;
-      if (last == 0) {  // the row's only part is its output
-        out[bh * D + d] = f2bf(L == 0.f ? 0.f : acc / L);
+      if (last == 0) {  // the row's only part is its output (keys that all score -inf leave 0 / 0)
+        out[bh * D + d] = f2bf(n ? acc / L : 0.f);
       } else {
         part_o[(bh * nparts + part) * D + d] = acc;
         if (d == 0) part_ml[(bh * nparts + part) * 2] = M, part_ml[(bh * nparts + part) * 2 + 1] = L;
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(C* G)
 #pragma unroll
     for (int i = 0; i < G; ++i) acc += sums[i][threadIdx.x];
   }
-  out[bh * D + d] = f2bf(L == 0.f ? 0.f : acc / L);
+  out[bh * D + d] = f2bf(n ? acc / L : 0.f);
 }
 
 }  // namespace mx

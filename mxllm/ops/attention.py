@@ -137,6 +137,12 @@ def _owned(w: torch.Tensor) -> bool:
     return w.is_leaf and any(hasattr(w, a) for a in ("_mx_grad32", "_mx_grad_fresh", "_mx_on_grad_ready"))
 
 
+def _check_capture(*leaves: torch.Tensor) -> None:
+    """Refuses a capture that these leaves' gradients cannot be part of (as the op's own autograd does)."""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        native().grads_capturable(leaves)
+
+
 def _norm_grads(ctx, dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad):
     """(d(qkv), dw_q, dw_k for autograd) of ``qk_norm_rope``: a weight with an owner that keeps its gradient (a trainer)
     takes it from the f32 sums with one rounding, None for autograd then."""
@@ -204,6 +210,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
         if _owned(q_norm) or _owned(k_norm):
+            _check_capture(qkv, q_norm, k_norm)
             return _QKNormRopeFn.apply(rows16(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
         return native().qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
     return ref.qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
@@ -219,6 +226,7 @@ def attention_block(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, B: 
     if norms is not None:
         wq, wk, eps = norms
         if use_native(qkv):
+            _check_capture(qkv, wq, wk)
             return _NormAttnBlockFn.apply(rows16(qkv), wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad)
         q, k, v = ref.qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps)
         return ref.attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal=causal).reshape(B * S, Hq * D)

@@ -221,7 +221,7 @@ def test_attention_of_long_and_uneven_rows(gpu, D, Hq, Hkv, lens):
 
 
 @pytest.mark.parametrize("B,hi", [(64, 700), (64, 2100), (20, 900), (130, 1000)])
-def test_attention_of_whole_rows_of_4_8_and_16_waves(gpu, B, hi):
+def test_attention_of_whole_rows_of_4_and_8_waves(gpu, B, hi):
     g = torch.Generator().manual_seed(B)
     lens = torch.randint(0, hi, (B,), generator=g).tolist()
     _check_attention(gpu, lens + [hi], 16, 8, 256, 64, seed=B)
@@ -275,6 +275,22 @@ def test_nan_keys_of_one_row_stay_with_it(gpu):
     p.k[int(p.table[1, 1]), 0, 7, 5] = 0x7F
     o = kv8.decode_attention(q, p, _i32([699] * 3, gpu), None, 700).view(3, 4, 64)
     assert o[1, :2].isnan().all() and torch.equal(o[1, 2:], good[1, 2:]) and torch.equal(o[0], good[0]) and torch.equal(o[2], good[2])
+
+
+@pytest.mark.parametrize("lens", [[40, 40], [5000, 40]])
+def test_scores_that_are_all_minus_infinity_have_no_softmax(gpu, lens):
+    D, Hq, Hkv = 64, 4, 2
+    p, q, good = _check_attention(gpu, lens, Hq, Hkv, 256, D)
+    for x in (p.k, p.v):
+        x.fill_(0x38)  # 1
+    p.k_exp.fill_(127)
+    p.v_exp.fill_(127)
+    q[:, 1, 7] = -torch.inf
+    args = (_i32([n - 1 for n in lens], gpu), None, max(lens))
+    o = kv8.decode_attention(q, p, *args).view(2, Hq, D)
+    assert o[:, 1].isnan().all() and bool((o[:, [0, 2, 3]] == 1).all())
+    plain = kv8.decode_attention(q.cpu(), kv8.Pages(*(t.cpu() for t in p)), _i32([n - 1 for n in lens]), None, max(lens))
+    assert torch.equal(plain.view(2, Hq, D).isnan(), o.isnan().cpu())
 
 
 def test_the_same_call_has_the_same_bits_captured_and_on_another_stream(gpu):
@@ -384,6 +400,24 @@ def test_refusals(gpu):
     with pytest.raises(RuntimeError):
         kv8.read(p, i32, i32, i32, -1)
     assert _same(before, p)
+
+
+def test_weights_tables_and_runs_at_odd_places(gpu):
+    """Copied, as rows there are: 16 bytes at a time is how they are read."""
+    D, Hq, Hkv, block = 64, 4, 2, 32
+    cos, sin = (t.to(gpu) for t in _tables(40, D))
+    qkv = _rows(33, Hq, Hkv, D).to(gpu)
+    wq, wk = ((1 + 0.1 * torch.randn(D)).bfloat16().to(gpu) for _ in range(2))
+    runs = kv8.prompt_runs([0], [33], [0], gpu)
+
+    def odd(t):
+        return torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape)
+
+    got = []
+    for place in (lambda t: t, odd):
+        p = kv8.Pages.empty(2, Hkv, block, D, _i32([[0, 1]], gpu))
+        got.append([*kv8.append_prompts(qkv, place(cos), place(sin), place(runs), p, Hq, place(wq), place(wk)), *p[:4]])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
 def test_no_rows(gpu):

@@ -179,6 +179,23 @@ def test_one_weight_for_both_norms_and_rows_at_odd_places(gpu):
 
 
 @pytest.mark.gpu
+def test_weights_tables_and_gradients_at_odd_places(gpu):
+    B, S, Hq, Hkv, D = 2, 9, 4, 2, 64
+    (qkv, *rest), cos, sin = _inputs(gpu, B, S, Hq, Hkv, D)
+
+    def odd(t):
+        return torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape)
+
+    got = []
+    for place in (lambda t: t, odd):
+        wq, wk, *grads = map(place, rest)
+        leaves = [t.detach().requires_grad_() for t in (qkv, wq, wk)]
+        out = ops.qk_norm_rope(*leaves, place(cos), place(sin), B, S, Hq, Hkv, D)
+        got.append([*out, *torch.autograd.grad(out, leaves, grads)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
 def test_no_rows_and_positions_outside_the_table(gpu):
     Hq, Hkv, D = 4, 2, 64
     (qkv, wq, wk, *_), cos, sin = _inputs(gpu, 0, 5, Hq, Hkv, D, table=4)
@@ -216,6 +233,31 @@ def test_captured_and_on_another_stream(gpu):
         want = step(qkv * (i + 1))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+@pytest.mark.parametrize("block", [False, True])
+def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused(gpu, block):
+    B, S, Hq, Hkv, D = 1, 40, 4, 2, 64
+    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, B, S, Hq, Hkv, D)
+    leaves = [t.detach().requires_grad_() for t in (qkv, wq, wk)]
+
+    def step():
+        if block:
+            return ops.attention_block(leaves[0], cos, sin, B, S, Hq, Hkv, D, norms=(*leaves[1:], EPS))
+        return ops.qk_norm_rope(*leaves, cos, sin, B, S, Hq, Hkv, D)
+
+    alive = step()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), capture_error_mode="thread_local"):
+            step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"), torch.no_grad():
+        got = step()  # (without a backward there is nothing to refuse)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*((x,) if block else x for x in (alive, got))))
 
 
 @pytest.mark.gpu
