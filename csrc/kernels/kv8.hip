@@ -19,6 +19,10 @@
 
 namespace mx {
 
+// A lane's P numbers of a head's half are pieces of 8 (4 where P is 4), of neighbouring lanes side by side: the second piece is
+// four pieces further.
+__device__ __forceinline__ constexpr int piece(int i) { return i / 8 * 32 + i % 8; }
+
 template <int P>
 __device__ __forceinline__ void load_bf(const uint16_t* p, float (&x)[P]) {
   if constexpr (P == 4) {
@@ -28,7 +32,7 @@ __device__ __forceinline__ void load_bf(const uint16_t* p, float (&x)[P]) {
   } else {
 #pragma unroll
     for (int i = 0; i < P; i += 8) {
-      const u16x8 v = *reinterpret_cast<const u16x8*>(p + i);
+      const u16x8 v = *reinterpret_cast<const u16x8*>(p + piece(i));
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[i + j] = bf2f(v[j]);
     }
@@ -47,7 +51,7 @@ __device__ __forceinline__ void store_bf(uint16_t* p, const float (&x)[P]) {
       u16x8 v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = f2bf(x[i + j]);
-      *reinterpret_cast<u16x8*>(p + i) = v;
+      *reinterpret_cast<u16x8*>(p + piece(i)) = v;
     }
   }
 }
@@ -55,36 +59,32 @@ template <int P>
 __device__ __forceinline__ void load_f32(const float* p, float (&x)[P]) {
 #pragma unroll
   for (int i = 0; i < P; i += 4) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p + piece(i));
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[i + j] = v[j];
   }
 }
-template <int P>
-struct CodeWords {
-  typedef uint32_t type __attribute__((ext_vector_type(P / 4)));
-};
-template <>
-struct CodeWords<4> {
-  typedef uint32_t type;
-};
+typedef uint32_t u32x2c __attribute__((ext_vector_type(2)));
 template <int P>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[P], int s) {
-  typename CodeWords<P>::type w;
-  if constexpr (P == 4) w = kv8_code4(x[0], x[1], x[2], x[3], s);
+  if constexpr (P == 4) *reinterpret_cast<uint32_t*>(p) = kv8_code4(x[0], x[1], x[2], x[3], s);
   else {
 #pragma unroll
-    for (int i = 0; i < P / 4; ++i) w[i] = kv8_code4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], s);
+    for (int i = 0; i < P; i += 8)
+      *reinterpret_cast<u32x2c*>(p + piece(i)) = u32x2c{kv8_code4(x[i], x[i + 1], x[i + 2], x[i + 3], s),
+                                                        kv8_code4(x[i + 4], x[i + 5], x[i + 6], x[i + 7], s)};
   }
-  *reinterpret_cast<typename CodeWords<P>::type*>(p) = w;
 }
 template <int P>
 __device__ __forceinline__ void load_codes(const uint8_t* p, float (&x)[P], int s) {
-  const auto w = *reinterpret_cast<const typename CodeWords<P>::type*>(p);
-  if constexpr (P == 4) kv8_value4(w, s, x);
+  if constexpr (P == 4) kv8_value4(*reinterpret_cast<const uint32_t*>(p), s, x);
   else {
 #pragma unroll
-    for (int i = 0; i < P / 4; ++i) kv8_value4(w[i], s, x + 4 * i);
+    for (int i = 0; i < P; i += 8) {
+      const u32x2c w = *reinterpret_cast<const u32x2c*>(p + piece(i));
+      kv8_value4(w[0], s, x + i);
+      kv8_value4(w[1], s, x + i + 4);
+    }
   }
 }
 // x by the nearest f32 with an odd last bit where f32 does not hold it: rounded to fewer bits afterwards, as x itself would be
@@ -102,13 +102,16 @@ __device__ __forceinline__ double lane_sum(double v) {
   const uint64_t other = ((uint64_t)lane_dpp<C>((uint32_t)(b >> 32)) << 32) | lane_dpp<C>((uint32_t)b);
   return v + __builtin_bit_cast(double, other);
 }
-// a, b: the pairs' halves; n = x r w (w null: x), turned by the angles of cos, sin; T: float or double.  Eight pairs at a time: 16
-// in flight in 64 bits take 244 registers, two waves a SIMD (a prompt of 4096 rows of 48 heads of 128 31.6 us, so 29.3; four
-// waves a SIMD, with registers in memory, 40).
+// a, b: the pairs' halves; n = x r w (w null: x), turned by the angles of cos, sin; T: float or double.  N pairs at a time, the
+// next ones' angles and weights not asked for before these are done (the compiler would put the products off until all
+// are there, 152 registers, 244 with 16 pairs at a time): 122 registers, four waves a SIMD, with 128 channels, 74 and six with
+// 64.  4,096 rows of 48 heads of 128 26.3 us (16 pairs at a time 31.6, 4 27.5), six prompts of 17 to 901 rows of 48 heads of 64 9.1
+// (8 at a time 10.0).
 template <typename T, int P>
 __device__ __forceinline__ void norm_turn(float (&a)[P], float (&b)[P], const uint16_t* w, int half, const float* cosb,
                                           const float* sinb, T eps) {
-  constexpr int N = P < 8 ? P : 8;
+  constexpr int N = P < 16 ? 4 : 8;
+  static_assert(P % N == 0 && (N % 8 == 0 || P <= 8), "whole pieces, or parts of the only one");
   T r = 1;
   if (w) {
     T ss = 0;
@@ -125,11 +128,11 @@ __device__ __forceinline__ void norm_turn(float (&a)[P], float (&b)[P], const ui
 #pragma unroll
   for (int p = 0; p < P; p += N) {
     float cs[N], sn[N], w1[N], w2[N];
-    load_f32<N>(cosb + p, cs);
-    load_f32<N>(sinb + p, sn);
+    load_f32<N>(cosb + piece(p), cs);
+    load_f32<N>(sinb + piece(p), sn);
     if (w) {
-      load_bf<N>(w + p, w1);
-      load_bf<N>(w + half + p, w2);
+      load_bf<N>(w + piece(p), w1);
+      load_bf<N>(w + half + piece(p), w2);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) w1[j] = w2[j] = 1.f;
@@ -145,7 +148,10 @@ __device__ __forceinline__ void norm_turn(float (&a)[P], float (&b)[P], const ui
         b[p + j] = rope_hi(x, y, c, s);
       }
     }
-    if (sizeof(T) == 8 && P > N) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (P > N) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) asm volatile("" : "+v"(a[p + j]), "+v"(b[p + j]));
+    }
   }
 }
 // |x| where it is a number
@@ -167,7 +173,7 @@ __global__ void __launch_bounds__(256)
   constexpr int P = D / 8, HALF = D / 2;
   const int Hkv = pg.Hkv, NH = Hq + 2 * Hkv;
   int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, row = lane >> 2, c = P * (lane & 3);
+  const int lane = threadIdx.x & 63, row = lane >> 2, c = (P < 8 ? P : 8) * (lane & 3);
   const int cap = (int)min((int64_t)pg.maxp * pg.block, (int64_t)turns);  // positions that a sequence can have
   if constexpr (!RUNS) {
     // single tokens: the first waves have 16 query heads each, of whatever rows, the others a key or value head of a row
@@ -291,7 +297,7 @@ __global__ void __launch_bounds__(256)
   const uint32_t per = (n + kUnit - 1) / kUnit;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= (int64_t)B * pg.Hkv * per) return;
-  const int i = (int)(item % per) * kUnit + ((threadIdx.x & 63) >> 2), c = P * (threadIdx.x & 3);
+  const int i = (int)(item % per) * kUnit + ((threadIdx.x & 63) >> 2), c = (P < 8 ? P : 8) * (threadIdx.x & 3);
   const int hk = (int)(item / per % pg.Hkv), b = (int)(item / per / pg.Hkv);
   if (i >= n) return;
   const int slot = slots ? slots[b] : b;
