@@ -19,8 +19,9 @@
 //   a lane's rows straight to registers, kept in the caches    32 x 100 .. 2000 of 128 19.6 / 16.6, 8 x 16384 54.9 / 54.6
 //   the same, not kept (rows of half a line: 40 x 1000 .. 4000 of 64 18.2 -> 19.7)      20.6 / 20.0,            49.8 / 49.3
 //   whole rows by LDS, not kept                                                        18.2 / 17.4,            49.8 / 48.9
-//   and the next tile on its way                                                       16.8 / 15.9,            49.2 / 48.7
-// and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 67.3 cold, 6.0 TB/s; one of 700 keys does not mind.
+//   and the next tile on its way                                                       16.1 / 15.4,            49.0 / 48.3
+// and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 66.7 cold, 6.1 TB/s; one of 700 keys does not mind.  (Keys of the tile after
+// next asked for as soon as a tile's are read, values alike, was 2 to 8 % slower.)
 //
 // Rows are whole (a workgroup each, nothing to merge) or cut: the units of all sequences in a row are dealt in equal
 // shares, one a workgroup of a KV head, whose four waves share what it has of a sequence, and sequences that were cut are
@@ -98,67 +99,101 @@ struct Kv8State {  // of one wave
     }
   };
 
-  // Two units' keys (32 rows) to LDS, then their values: k0, v0 / k1, v1: the units; ALL: every row of both is there; else lim: their
-  // last one (less than 0: none), and rows behind it are read as that row.  As the products want them, a lane a row, a load would
-  // ask for 64 pieces of as many lines; so it has whole rows, 1 KB.
+  // A unit's keys or values (16 rows) to LDS; ALL: every row of it is there; else lim: its last one (less than 0: none), and rows
+  // behind it are read as that row.  As the products want them, a lane a row, a load would ask for 64 pieces of as many lines;
+  // so it has whole rows, 1 KB.
   template <bool ALL>
-  static __device__ __forceinline__ void load(char* lds, const uint8_t* __restrict__ k0, const uint8_t* __restrict__ k1,
-                                              const uint8_t* __restrict__ v0, const uint8_t* __restrict__ v1, int lim0,
-                                              int lim1, int lane) {
-    constexpr int N = D / 16, ROWS = 64 / N;  // of a load
-    const int z0 = max(lim0, 0), z1 = max(lim1, 0);
+  static __device__ __forceinline__ void load(char* lds, const uint8_t* unit, int lim, int lane) {
+    constexpr int N = D / 16, ROWS = 64 / N;  // pieces of a row, rows of a load
+    static_assert(D >= 64, "a load of one unit");
+    const int r = lane / N, at = 16 * ((place(r, lane % N) - r * D) / 16);  // (the exchange is its own inverse)
+    if constexpr (ALL) {
+      asm("" : "+s"(unit));  // (a base for all lanes, not added to each one's offset)
+      __builtin_amdgcn_global_load_lds((gptr_t)(unit + (uint32_t)(r * D + at)), (lptr_t)lds, 16, 0, kNt);
+      if constexpr (ROWS == 8)  // rows 8 further change places alike
+        __builtin_amdgcn_global_load_lds((gptr_t)(unit + (uint32_t)(r * D + at)), (lptr_t)lds, 16, 1024, kNt);
+    } else {
+      const int z = max(lim, 0);
 #pragma unroll
-    for (int i = 0; i < 64 / ROWS; ++i) {
-      const bool val = i >= 32 / ROWS;
-      const int row = ROWS * (val ? i - 32 / ROWS : i) + lane / N, r = row & 15;
-      const bool second = ROWS == 32 ? lane >= 32 : (ROWS * i & 31) >= 16;
-      const int ch = (place(row, lane % N) - row * D) / 16;  // (the exchange is its own inverse)
-      const uint8_t* p = (val ? second ? v1 : v0 : second ? k1 : k0) + (uint32_t)((ALL ? r : min(r, second ? z1 : z0)) * D + 16 * ch);
-      __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(lds + 1024 * i), 16, 0, kNt);
+      for (int i = 0; i < 16 / ROWS; ++i)
+        __builtin_amdgcn_global_load_lds((gptr_t)(unit + (uint32_t)(min(ROWS * i + r, z) * D + at)), (lptr_t)(lds + 1024 * i),
+                                         16, 0, kNt);
+    }
+  }
+  // Both units of a tile, keys and values (rows of 32 bytes: a load has both units')
+  template <bool ALL>
+  static __device__ __forceinline__ void load_tile(char* lds, const uint8_t* k0, const uint8_t* k1, const uint8_t* v0,
+                                                   const uint8_t* v1, int lim0, int lim1, int lane) {
+    if constexpr (D == 32) {
+      const int row = lane / 2, z = max(lane < 32 ? lim0 : lim1, 0);
+      const uint32_t off = (ALL ? row & 15 : min(row & 15, z)) * D + 16 * (lane % 2);
+      __builtin_amdgcn_global_load_lds((gptr_t)((lane < 32 ? k0 : k1) + off), (lptr_t)lds, 16, 0, kNt);
+      __builtin_amdgcn_global_load_lds((gptr_t)((lane < 32 ? v0 : v1) + off), (lptr_t)(lds + 1024), 16, 0, kNt);
+    } else {
+      load<ALL>(lds, k0, lim0, lane);
+      load<ALL>(lds + 16 * D, k1, lim1, lane);
+      load<ALL>(lds + 32 * D, v0, lim0, lane);
+      load<ALL>(lds + 48 * D, v1, lim1, lane);
     }
   }
 
-  // ks: what the units' scores are multiplied by, vs: powers of two of their values
-  template <bool ALL, int OFF>
-  __device__ __forceinline__ void take(const Places& at, const u16x8 (&qf)[KS], float ks0, float ks1, float vs0, float vs1,
-                                       int lim0, int lim1, int c, int g) {
+  // off: the tile's half; ks: what the units' scores are multiplied by, vs: powers of two of their values; all: every row is
+  // there, else up to lim0, lim1
+  __device__ __forceinline__ void take(const Places& from, uint32_t off, const u16x8 (&qf)[KS], float ks0, float ks1,
+                                       float vs0, float vs1, bool all, int lim0, int lim1, int c, int g) {
+    Places at = from;
+#pragma unroll
+    for (uint32_t& x : at.k) x += off;
+#pragma unroll
+    for (uint32_t& x : at.v) x += off;
     f32x4 sc[2];
+    typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
     // (one block of reads and their wait: the compiler would wait for the next tile, which is on its way to the other half)
-    if constexpr (D == 128) {
-      u32x4v w0, w1, w2, w3;
-      asm volatile("ds_read_b128 %0, %4 offset:%6\n\tds_read_b128 %1, %5 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\t"
-                   "ds_read_b128 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(w0), "=&v"(w1), "=&v"(w2), "=&v"(w3)
-                   : "v"(at.k[0]), "v"(at.k[1]), "i"(OFF), "i"(OFF + 16 * D)
-                   : "memory");
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[2], w0[3])), qf[1], sc[0]);
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[2], w2[3])), qf[1], sc[1]);
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[0], w1[1])), qf[2], sc[0]);
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[0], w3[1])), qf[2], sc[1]);
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[2], w1[3])), qf[3], sc[0]);
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[2], w3[3])), qf[3], sc[1]);
-    } else if constexpr (D == 64) {
-      u32x4v w0, w2;
-      asm volatile("ds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(w0), "=&v"(w2) : "v"(at.k[0]), "i"(OFF), "i"(OFF + 16 * D) : "memory");
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
-      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[2], w0[3])), qf[1], sc[0]);
-      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[2], w2[3])), qf[1], sc[1]);
-    } else {
+#define KV8_V(OP)                                                                                       \
+  OP " %[v0], %[b0]\n\t" OP " %[v1], %[b1]\n\t" OP " %[v2], %[b2]\n\t" OP " %[v3], %[b3]\n\t"             \
+  OP " %[v4], %[b0] offset:%[p]\n\t" OP " %[v5], %[b1] offset:%[p]\n\t" OP " %[v6], %[b2] offset:%[p]\n\t" \
+  OP " %[v7], %[b3] offset:%[p]\n\ts_waitcnt lgkmcnt(0)"
+#define KV8_V_OUT                                                                                             \
+  [v0] "=&v"(v[0]), [v1] "=&v"(v[1]), [v2] "=&v"(v[2]), [v3] "=&v"(v[3]), [v4] "=&v"(v[4]), [v5] "=&v"(v[5]), \
+      [v6] "=&v"(v[6]), [v7] "=&v"(v[7])
+#define KV8_V_IN [b0] "v"(at.v[0]), [b1] "v"(at.v[1]), [b2] "v"(at.v[2]), [b3] "v"(at.v[3]), [p] "i"(16 * D)
+    if constexpr (D == 32) {
       u32x2v w0, w2;
-      asm volatile("ds_read_b64 %0, %2 offset:%3\n\tds_read_b64 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(w0), "=&v"(w2) : "v"(at.k[0]), "i"(OFF), "i"(OFF + 16 * D) : "memory");
+      asm volatile("ds_read_b64 %[w0], %[a0]\n\tds_read_b64 %[w2], %[a0] offset:%[p]\n\t" KV8_V("ds_read_u16")
+                   : [w0] "=&v"(w0), [w2] "=&v"(w2), KV8_V_OUT : [a0] "v"(at.k[0]), KV8_V_IN : "memory");
       sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
       sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+    } else {
+      u32x4v w0, w1, w2, w3;
+      if constexpr (D == 128)
+        asm volatile("ds_read_b128 %[w0], %[a0]\n\tds_read_b128 %[w2], %[a0] offset:%[p]\n\t"
+                     "ds_read_b128 %[w1], %[a1]\n\tds_read_b128 %[w3], %[a1] offset:%[p]\n\t" KV8_V("ds_read_b64")
+                     : [w0] "=&v"(w0), [w1] "=&v"(w1), [w2] "=&v"(w2), [w3] "=&v"(w3), KV8_V_OUT
+                     : [a0] "v"(at.k[0]), [a1] "v"(at.k[1]), KV8_V_IN
+                     : "memory");
+      else
+        asm volatile("ds_read_b128 %[w0], %[a0]\n\tds_read_b128 %[w2], %[a0] offset:%[p]\n\t" KV8_V("ds_read_b32")
+                     : [w0] "=&v"(w0), [w2] "=&v"(w2), KV8_V_OUT : [a0] "v"(at.k[0]), KV8_V_IN : "memory");
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[0], w0[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[0], w2[1])), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w0[2], w0[3])), qf[1], sc[0]);
+      sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w2[2], w2[3])), qf[1], sc[1]);
+      if constexpr (D == 128) {
+        sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[0], w1[1])), qf[2], sc[0]);
+        sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[0], w3[1])), qf[2], sc[1]);
+        sc[0] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w1[2], w1[3])), qf[3], sc[0]);
+        sc[1] = mfma16(__builtin_bit_cast(u32x4v, dequant8(w3[2], w3[3])), qf[3], sc[1]);
+      }
     }
+#undef KV8_V
+#undef KV8_V_OUT
+#undef KV8_V_IN
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = sc[i >> 2][i & 3] * (i < 4 ? ks0 : ks1);
-      if (!ALL) x[i] = 4 * g + (i & 3) <= (i < 4 ? lim0 : lim1) ? x[i] : -INFINITY;
+    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * (i < 4 ? ks0 : ks1);
+    if (!all) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 4 * g + (i & 3) <= (i < 4 ? lim0 : lim1) ? x[i] : -INFINITY;
     }
     // The exponents' reference is a maximum that may be behind by 2^8: weights up to there cost no precision, and the sums are
     // multiplied again in a few of the tiles only
@@ -180,18 +215,6 @@ struct Kv8State {  // of one wave
       l += p;
       pb[i] = f2bf(p);
     }
-    typename VPiece<E>::type v[8];  // slot s: row 4 g + (s & 3) of unit s >> 2, channels E c ..
-#define KV8_READ8(OP)                                                                                                     \
-  asm volatile(OP " %0, %8 offset:%12\n\t" OP " %1, %9 offset:%12\n\t" OP " %2, %10 offset:%12\n\t" OP " %3, %11 offset:%12\n\t" \
-               OP " %4, %8 offset:%13\n\t" OP " %5, %9 offset:%13\n\t" OP " %6, %10 offset:%13\n\t" OP " %7, %11 offset:%13\n\t" \
-               "s_waitcnt lgkmcnt(0)"                                                                                      \
-               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])    \
-               : "v"(at.v[0]), "v"(at.v[1]), "v"(at.v[2]), "v"(at.v[3]), "i"(OFF), "i"(OFF + 16 * D)                       \
-               : "memory")
-    if constexpr (D == 128) KV8_READ8("ds_read_b64");
-    else if constexpr (D == 64) KV8_READ8("ds_read_b32");
-    else KV8_READ8("ds_read_u16");
-#undef KV8_READ8
     // bytes 0, 1 or 2, 3 of the words of two rows side by side, as pairs of rows of one channel each
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
@@ -305,40 +328,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const float vs = __uint_as_float((uint32_t)pg.ve[where] << 23);
       const int tiles = min(32, (u1 - t0 + 2 * WAVES - 1) / (2 * WAVES));  // of this wave, here
       const int whole = min(u1, len / kUnit);                                // units before this one have all their rows
-      const auto all = [&](int i) { return t0 + 2 * WAVES * i + 2 <= whole; };
       const auto fetch = [&](int i, int half) {
         const int64_t a0 = (int64_t)__builtin_amdgcn_readlane(where, 2 * i) * (kUnit * D);
         const int64_t a1 = (int64_t)__builtin_amdgcn_readlane(where, 2 * i + 1) * (kUnit * D);
         const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
         char* to = kl + half * (64 * D);
-        if (all(i)) State::template load<true>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, 15, 15, lane);
-        else State::template load<false>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, lane);
+        if (u + 2 <= whole) State::template load_tile<true>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, 15, 15, lane);
+        else State::template load_tile<false>(to, pg.k + a0, pg.k + a1, pg.v + a0, pg.v + a1, lim, lim1, lane);
       };
-      const auto use = [&](int i, auto off) {
-        constexpr int OFF = decltype(off)::value;
-        const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
-        const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
-        if (all(i)) st.template take<true, OFF>(at, qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), 15, 15, c, g);
-        else st.template take<false, OFF>(at, qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), lim, lim1, c, g);
-      };
+      const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
       constexpr int LOADS = D / 16;  // of a tile
       fetch(0, 0);
-      for (int i = 0; i < tiles; i += 2) {
+      for (int i = 0; i < tiles; ++i) {
         if (i + 1 < tiles) {
-          fetch(i + 1, 1);
+          fetch(i + 1, (i + 1) & 1);
           __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);  // the older tile has landed (only this wave reads it)
         } else {
           __builtin_amdgcn_s_waitcnt(0x0F70);
         }
-        use(i, std::integral_constant<int, 0>{});
-        if (i + 1 >= tiles) break;
-        if (i + 2 < tiles) {
-          fetch(i + 2, 0);
-          __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);
-        } else {
-          __builtin_amdgcn_s_waitcnt(0x0F70);
-        }
-        use(i + 1, std::integral_constant<int, 64 * D>{});
+        const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
+        st.take(at, (i & 1) * (64 * D), qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), u + 2 <= whole,
+                lim, lim1, c, g);
       }
     }
     st.l = lane_sum<32>(lane_sum<16>(st.l));
@@ -453,15 +463,18 @@ __global__ void __launch_bounds__(C* G)
 using namespace mx;
 
 // Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB (a CU's 60 GB/s,
-// whatever its waves); cutting costs a merge and more ends, 4 to 9 us.  Us with whole rows of 4 / 8 waves, and cut:
-//   1 x 700 keys, 8 heads of 64 5.7 / 5.1, 7.3; of 128 7.5 / 6.6, 8.7;  1 x 4096 of 128 25.6 / 18.6, 10.9
-//   16 x 500 .. 2000, 8 heads of 64 11.5 / 9.5, 13.4;  40 x 1000 .. 4000, 5 heads of 64 20.3 / 15.5, 20.4
-//   32 x 100 .. 2000, 8 heads of 128 16.6 / 16.1, 22.0;  64 x 30 .. 512 10.0 / 12.5, 18.1;  64 x 2048 .. 4096 68.9 / 70.2, 74.4
+// however many waves); cutting costs a merge and more ends, 4 to 9 us.  Rows that leave no CU alone are better off by four
+// waves, where a CU has the next row's workgroup beside this one's end.  Us with whole rows of 4 / 8 waves, and cut:
+//   heads of 128: 8 rows of 700 keys 6.9 / 6.4, 8.4; of 4,096 22.5 / 18.0, 10.8;  64 of 16,384 88.8 / 84.7, 48.4;  192 of 100 .. 2000
+//     14.3 / 14.7, 18.5;  256 15.5 / 15.9, 20.4;  320 21.1 / 22.4, 22.0;  512 of 30 .. 512 9.6 / 12.1, 17.0;  of 2048 .. 4096 67.6 / 70.6, 74.3
+//   of 64: 8 of 700 5.7 / 5.0, 7.5;  128 of 500 .. 2000 11.3 / 9.1, 13.5;  200 of 1000 .. 4000 20.0 / 15.2, 20.5;  384 of 100 .. 2000
+//     13.6 / 14.3, 18.6;  512 of 30 .. 512 6.9 / 7.2, 16.0;  of 2048 .. 4096 35.5 / 35.4, 42.0
+//   of 32: 64 of 4096 .. 8192 30.5 / 19.1, 13.2;  512 of 1000 .. 8000 38.7 / 34.2, 37.5;  1,024 of 1000 .. 4000 31.7 / 31.0, 40.5
 // Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 10 us.
 static int kv8_waves(int64_t rows, int64_t cap, int D) {
   const int64_t bytes = cap * D;  // of keys
   if (bytes > (rows >= 384 ? 524288 : rows >= 128 ? 262144 : 131072)) return 0;
-  return rows >= 384 ? 4 : 8;
+  return rows * D >= 192 * 128 ? 4 : 8;
 }
 // workgroups of a KV head where keys are dealt evenly: two a CU of 256
 static int kv8_shares(int Hkv) { return Hkv < 512 ? (512 + Hkv - 1) / Hkv : 1; }

@@ -220,11 +220,12 @@ def test_attention_of_long_and_uneven_rows(gpu, D, Hq, Hkv, lens):
     _check_attention(gpu, lens, Hq, Hkv, 256, D, seed=len(lens))
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("B,hi", [(64, 700), (64, 2100), (20, 900), (130, 1000)])
-def test_attention_of_whole_rows_of_4_and_8_waves(gpu, B, hi):
+def test_attention_of_whole_rows_of_4_and_8_waves(gpu, B, hi, D):
     g = torch.Generator().manual_seed(B)
     lens = torch.randint(0, hi, (B,), generator=g).tolist()
-    _check_attention(gpu, lens + [hi], 16, 8, 256, 64, seed=B)
+    _check_attention(gpu, lens + [hi], 16, 8, 256, D, seed=B)
 
 
 @pytest.mark.parametrize("size", [2.0 ** -60, 1.0, 2.0 ** 60])
