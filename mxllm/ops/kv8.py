@@ -31,7 +31,8 @@ E4M3_MAX = 448.0
 class Pages(NamedTuple):
     """One layer's cache and the block table: position p of slot s lies in page ``table[s, p // block]`` at row
     ``p % block``.  Kernels look at no page outside the pool: what a sequence has there is not written, and comes
-    back, from a read or through attention, as NaN."""
+    back, from a read or through attention, as NaN.  Slots may share pages that they read; a group of positions that two of them
+    append to in one call is the callers' to prevent."""
 
     k: torch.Tensor  # uint8 [pages, Hkv, block, D]
     v: torch.Tensor

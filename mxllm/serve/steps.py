@@ -55,9 +55,11 @@ class LlamaSteps:
         scratch = eng.scratch_slot if eng.use_graphs else None
         self.kv8 = eng.kv_dtype == "e4m3"
         if self.kv8:
-            if eng.device.type == "cuda" and (c.head_dim not in (32, 64, 128) or c.n_heads // c.n_kv_heads > 16):
-                raise ValueError(f"kv_dtype e4m3: heads of 32, 64 or 128 channels, up to 16 a key head, not {c.head_dim}, "
-                                 f"{c.n_heads // c.n_kv_heads}")
+            dtype = self.model.tok_emb.dtype
+            if eng.device.type == "cuda" and (c.head_dim not in (32, 64, 128) or c.n_heads // c.n_kv_heads > 16
+                                              or dtype != torch.bfloat16):
+                raise ValueError(f"kv_dtype e4m3: bf16 heads of 32, 64 or 128 channels, up to 16 a key head, not {dtype}, "
+                                 f"{c.head_dim}, {c.n_heads // c.n_kv_heads}")
             kv = KV8Cache(c.n_layers, c.n_kv_heads, c.head_dim, eng.device, n_slots, eng.max_seq, pool_tokens, block, scratch)
         else:
             kv = KVCache(c.n_layers, c.n_kv_heads, c.head_dim, self.model.tok_emb.dtype, eng.device, n_slots, eng.max_seq,

@@ -331,6 +331,25 @@ def test_the_same_call_has_the_same_bits_captured_and_on_another_stream(gpu):
         assert torch.equal(graphs[i % 2][1], want) and _same(mine, eager)
 
 
+def test_pages_past_32_bits(gpu):
+    """A pool whose last pages lie more than 4 GiB behind its first gives what a small one does."""
+    D, Hq, Hkv, block, n = 128, 16, 8, 256, 300
+    cos, sin = (t.to(gpu) for t in _tables(n + 2, D))
+    qkv, more = _rows(n, Hq, Hkv, D).to(gpu), _rows(1, Hq, Hkv, D, seed=5).to(gpu)
+    runs, pos, slots = kv8.prompt_runs([0], [n], [0], gpu), _i32([n], gpu), _i32([0], gpu)
+    out = []
+    for pages, table in ((3, [[2, 0]]), (17000, [[16999, 16500]])):
+        k, v = (torch.empty(pages, Hkv, block, D, dtype=torch.uint8, device=gpu) for _ in range(2))
+        ke, ve = (torch.zeros(pages, Hkv, block // 16, dtype=torch.uint8, device=gpu) for _ in range(2))
+        p = kv8.Pages(k, v, ke, ve, _i32(table, gpu))
+        kv8.append_prompts(qkv, cos, sin, runs, p, Hq)
+        q = kv8.append_tokens(more, cos, sin, pos, slots, p, Hq)
+        out.append([q, *kv8.read(p, slots, _i32([0], gpu), pos + 1, n + 1), kv8.decode_attention(q, p, pos, slots, n + 1),
+                    kv8.decode_attention(q, p, pos, slots, 4096)])
+        del p, k, v
+    assert 16500 * Hkv * block * D > 2 ** 32 and all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_prompt_then_tokens_is_attention_over_all(gpu):
     """What serving does: a prompt with normed heads appended, then token after token; each token's attention against 64 bits over
     what was appended.  Half a step of e4m3 (2^-4 of a value, or 2^-10 of the power of two that its group has) in keys moves a

@@ -126,6 +126,25 @@ def test_rows_of_a_wider_buffer_and_broadcast_gradients(gpu, D, Hq, Hkv):
 
 
 @pytest.mark.gpu
+def test_rows_past_32_bits(gpu):
+    """351 copies of 1,000 rows, 2^31 numbers and more: the last copy comes out, and goes back, as the rows alone do."""
+    B, S, Hq, Hkv, D, n = 8, 43875, 32, 8, 128, 1000
+    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, 1, n, Hq, Hkv, D)
+    pos = torch.randint(0, n, (n,), generator=torch.Generator().manual_seed(3)).int().to(gpu)
+    ends = []
+    for b, s in ((1, n), (B, S)):
+        rows = qkv.repeat(b * s // n, 1)
+        at = pos.repeat(b * s // n)
+        rows.requires_grad_()
+        out = ops.qk_norm_rope(rows, wq, wk, cos, sin, b, s, Hq, Hkv, D, EPS, at)
+        back = torch.autograd.grad(out, rows, [o.detach() for o in out])[0]
+        ends.append([*(o.detach()[-1, :, -n:].clone() for o in out), back[-n:].clone()])
+        assert b == 1 or rows.numel() > 2 ** 31
+        del rows, out, back
+    assert all(torch.equal(x, y) for x, y in zip(*ends))
+
+
+@pytest.mark.gpu
 def test_unused_outputs_and_frozen_weights(gpu):
     B, S, Hq, Hkv, D = 1, 21, 4, 2, 64
     (qkv, wq, wk, gq, gk, gv), cos, sin = _inputs(gpu, B, S, Hq, Hkv, D)
