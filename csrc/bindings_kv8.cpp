@@ -196,6 +196,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_grad(const at::Tenso
                                                                  const at::Tensor& wk, const at::Tensor& cos,
                                                                  const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq,
                                                                  int64_t Hkv, int64_t D, double eps, const OptTensor& positions) {
+  bool recorded = false;
+  for (const at::Tensor* t : {&qkv, &wq, &wk})
+    recorded = recorded || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
+  if (!recorded) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
+  }
   if (at::GradMode::is_enabled()) {
     DevGuard g(qkv.device());
     check_capture({qkv, wq, wk});

@@ -209,7 +209,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     the table ``cos``, ``sin`` [positions, D / 2] comes out as NaN.  Differentiable once, in qkv and both weights
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
-        if _owned(q_norm) or _owned(k_norm):
+        if (q_norm.requires_grad or k_norm.requires_grad) and (_owned(q_norm) or _owned(k_norm)):
             _check_capture(qkv, q_norm, k_norm)
             return _QKNormRopeFn.apply(rows16(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
         return native().qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)

@@ -255,6 +255,17 @@ def test_captured_and_on_another_stream(gpu):
 
 
 @pytest.mark.gpu
+def test_forward_mode_is_refused(gpu):
+    B, S, Hq, Hkv, D = 1, 6, 4, 2, 64
+    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, B, S, Hq, Hkv, D)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(qkv, torch.ones_like(qkv))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                ops.qk_norm_rope(dual, wq, wk, cos, sin, B, S, Hq, Hkv, D)
+
+
+@pytest.mark.gpu
 @pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 @pytest.mark.parametrize("block", [False, True])
 def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused(gpu, block):
