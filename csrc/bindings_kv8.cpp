@@ -297,7 +297,7 @@ std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& kc, const at::Tens
   const mx::Kv8Pages pg = check_pages(kc, vc, ke, ve, table, kc);
   const int64_t Hkv = kc.size(1), D = kc.size(3);
   check_heads(Hkv, Hkv, D);
-  MX_CHECK(starts.dim() == 1 && n >= 0 && n <= INT32_MAX, "starts int32 [B], n >= 0");
+  MX_CHECK(starts.dim() == 1 && n >= 0 && n <= INT32_MAX - 16, "starts int32 [B], n >= 0");
   const int64_t B = starts.size(0);
   const int32_t *from = check_ints(starts, {B}, kc, "starts"), *to = check_ints(ends, {B}, kc, "ends");
   const int32_t* sl = given(slots) ? check_ints(*slots, {B}, kc, "slots") : nullptr;
