@@ -330,13 +330,14 @@ at::Tensor kv8_decode_attn(const at::Tensor& q_any, const at::Tensor& kc, const 
   const int64_t cap = std::min<int64_t>(max_len, (int64_t)pg.maxp * pg.block);
   auto out = at::empty({B, Hq * D}, q.options());
   const int64_t parts = mx_kv8_attn_parts((int)B, (int)Hkv, (int)D, (int)cap);
-  at::Tensor ml, po;
+  at::Tensor work;  // outputs of the parts [B, Hq, parts, D], then their maxima and sums [B, Hq, parts, 2]
+  float *po = nullptr, *ml = nullptr;
   if (parts) {
-    ml = at::empty({B, Hq, parts, 2}, q.options().dtype(at::kFloat));
-    po = at::empty({B, Hq, parts, D}, q.options().dtype(at::kFloat));
+    work = at::empty({B * Hq * parts * (D + 2)}, q.options().dtype(at::kFloat));
+    po = work.data_ptr<float>(), ml = po + B * Hq * parts * D;
   }
-  const int rc = mx_kv8_attn(bf(q), &pg, p, sl, parts ? ml.data_ptr<float>() : nullptr, parts ? po.data_ptr<float>() : nullptr,
-                             bfm(out), (int)B, (int)Hq, (int)D, (int)cap, (float)scale, cur_stream());
+  const int rc = mx_kv8_attn(bf(q), &pg, p, sl, ml, po, bfm(out), (int)B, (int)Hq, (int)D, (int)cap, (float)scale,
+                             cur_stream());
   MX_CHECK(rc != -1, "kv8_decode_attn: sizes not taken");
   MX_OK(rc);
   return out;
