@@ -2,7 +2,7 @@
 //   o = softmax(q k^T scale) v over positions 0 .. pos, queries of a group of heads sharing a key/value head.
 //
 // Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
-// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 49 us, of which the merge 5; a linear read of as much takes 45.
+// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 49 us, of which the merge 4; a linear read of as much takes 45.
 //
 //   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
 // by v_mfma_f32_16x16x32_bf16 on codes that become bf16 in registers, where they are exact, the units' (16 positions) powers of
@@ -24,8 +24,8 @@
 // next asked for as soon as a tile's are read, values alike, was 2 to 8 % slower.)
 //
 // Rows are whole (a workgroup each, nothing to merge) or cut: the units of all sequences in a row are dealt in equal
-// shares, one a workgroup of a KV head, whose four waves share what it has of a sequence, and sequences that were cut are
-// merged by a second launch.  Where a row is cut follows from the lengths of all, so the last bits of an output may
+// shares, one a workgroup of a KV head, whose waves share what it has of a sequence, and sequences that were cut are merged by a
+// second launch.  Where a row is cut follows from the lengths of all, so the last bits of an output may
 // differ from batch to batch (the same call has the same bits).
 #include "kv8.h"
 
@@ -463,21 +463,26 @@ __global__ void __launch_bounds__(C* G)
 using namespace mx;
 
 // Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB (a CU's 60 GB/s,
-// however many waves); cutting costs a merge and more ends, 4 to 9 us.  Rows that leave no CU alone are better off by four
-// waves, where a CU has the next row's workgroup beside this one's end.  Us with whole rows of 4 / 8 waves, and cut:
-//   heads of 128: 8 rows of 700 keys 6.9 / 6.4, 8.4; of 4,096 22.5 / 18.0, 10.8;  64 of 16,384 88.8 / 84.7, 48.4;  192 of 100 .. 2000
-//     14.3 / 14.7, 18.5;  256 15.5 / 15.9, 20.4;  320 21.1 / 22.4, 22.0;  512 of 30 .. 512 9.6 / 12.1, 17.0;  of 2048 .. 4096 67.6 / 70.6, 74.3
-//   of 64: 8 of 700 5.7 / 5.0, 7.5;  128 of 500 .. 2000 11.3 / 9.1, 13.5;  200 of 1000 .. 4000 20.0 / 15.2, 20.5;  384 of 100 .. 2000
-//     13.6 / 14.3, 18.6;  512 of 30 .. 512 6.9 / 7.2, 16.0;  of 2048 .. 4096 35.5 / 35.4, 42.0
-//   of 32: 64 of 4096 .. 8192 30.5 / 19.1, 13.2;  512 of 1000 .. 8000 38.7 / 34.2, 37.5;  1,024 of 1000 .. 4000 31.7 / 31.0, 40.5
-// Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 10 us.
+// however many waves); cutting costs a merge and more ends, 2 to 7 us.  Rows that leave no CU alone are better off by four
+// waves, where a CU has the next row's workgroup beside this one's end.  Us, cold, with whole rows of 4 / 8 waves, and cut:
+//   heads of 128: 8 rows of 700 keys 7.5 / 7.2, 8.3; of 1,024 8.7 / 8.6, 8.4; of 2,048 13.4 / 13.2, 8.9;  32 of 1,500 11.4 / 11.5, 11.1;
+//     64 of 1000 .. 2000 13.7 / 13.9, 14.4; of 16,384 88.9 / 84.8, 49.5;  128 of 1000 .. 2000 14.6 / 15.1, 19.2; of 2000 .. 4096 24.8 / 25.6,
+//     26.1;  192 of 100 .. 4096 25.5 / 26.6, 27.2;  256 of 100 .. 2000 16.0 / 16.8, 21.3; of 100 .. 4096 27.4 / 28.4, 33.6;  512 of 30 .. 512
+//     10.6 / 12.8, 20.0; of 2048 .. 4096 66.8 / 70.1, 72.2
+//   of 64: 8 of 700 6.1 / 5.4, 7.5; of 2,048 11.3 / 8.9, 8.1;  64 of 1000 .. 3000 14.6 / 10.9, 12.4;  128 of 500 .. 2000 11.5 / 9.1, 13.9; of 1000
+//     .. 6000 29.2 / 19.6, 18.5;  192 of 100 .. 4000 20.0 / 14.8, 18.4;  320 of 1000 .. 8000 45.7 / 47.9, 39.6;  384 of 100 .. 2000 14.0 / 14.8,
+//     19.1;  512 of 2048 .. 4096 36.1 / 36.8, 42.5
+//   of 32: 64 of 4096 .. 8192 31.1 / 19.5, 13.2;  512 of 1000 .. 8000 39.5 / 35.9, 38.1;  1,024 of 30 .. 512 7.2 / 7.4, 18.8
+// Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 12 us.
 static int kv8_waves(int64_t rows, int64_t cap, int D) {
-  const int64_t bytes = cap * D;  // of keys
-  if (bytes > (rows >= 384 ? 524288 : rows >= 128 ? 262144 : 131072)) return 0;
-  return rows * D >= 192 * 128 ? 4 : 8;
+  if (cap > (rows >= 128 ? 4096 : rows >= 32 ? 32 * rows : 1024)) return 0;
+  return rows >= (D == 128 ? 128 : D == 64 ? 384 : 1024) ? 4 : 8;
 }
-// workgroups of a KV head where keys are dealt evenly: two a CU of 256
-static int kv8_shares(int Hkv) { return Hkv < 512 ? (512 + Hkv - 1) / Hkv : 1; }
+// Workgroups of a KV head where keys are dealt evenly: one a CU of 256, of four waves with heads of 128, of eight with smaller ones.
+// Us with 512 of four waves, 256 of eight, 256 of four: 8 rows (8 heads) of 128 of 4,096 keys 10.8, 10.4, 10.2, of 32,768 20.2, 18.8, 18.6;
+// 64 of 16,384 49.3, 50.1, 49.7; 512 of 500 .. 8192 94.6, 96.4, 93.3;  8 of 64 of 16,384 12.5, 11.0, 11.0; 64 of 4000 .. 8192 17.6, 17.7,
+// 18.1;  64 of 32 of 4096 .. 8192 13.7, 13.1, 14.4.  (768 of four waves 23.8 and 55.0 where 512 have 20.2 and 49.3.)
+static int kv8_shares(int Hkv) { return Hkv < 256 ? (256 + Hkv - 1) / Hkv : 1; }
 
 // parts that a row of up to `cap` keys can be cut into (of part_ml [B, Hq, parts, 2], part_o [B, Hq, parts, D]); 0: rows are whole
 extern "C" int mx_kv8_attn_parts(int B, int Hkv, int D, int cap) {
@@ -515,11 +520,12 @@ void launch(const Launch& a) {
     else launch_whole<D, 8>(a);
     return;
   }
-  kv8_attn_kernel<D, 4, true><<<dim3(W, Hkv), 256, 0, a.stream>>>(
+  constexpr int WAVES = D == 128 ? 4 : 8;
+  kv8_attn_kernel<D, WAVES, true><<<dim3(W, Hkv), 64 * WAVES, 0, a.stream>>>(
       a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages, Hkv,
       a.part_ml, a.part_o, a.out, a.B, a.Hq, a.cap, nparts, a.sl);
   const int rows = a.B * a.Hq;
-  if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.1 -> 10.4 us, 1 x 32768 34.9 -> 19.9
+  if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.5 -> 10.8 us, 1 x 32768 34.1 -> 20.3
     kv8_merge_kernel<D, 32, 8><<<rows * (D / 32), 256, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots, a.out, a.B,
                                                                       a.Hq, W, a.cap, nparts);
   else

@@ -221,7 +221,7 @@ def test_attention_of_long_and_uneven_rows(gpu, D, Hq, Hkv, lens):
 
 
 @pytest.mark.parametrize("D", [32, 64, 128])
-@pytest.mark.parametrize("B,hi", [(64, 700), (64, 2100), (20, 900), (130, 1000)])
+@pytest.mark.parametrize("B,hi", [(64, 700), (64, 2100), (20, 900), (130, 1000), (16, 4096), (16, 4200), (4, 1024), (7, 1800)])
 def test_attention_of_whole_rows_of_4_and_8_waves(gpu, B, hi, D):
     g = torch.Generator().manual_seed(B)
     lens = torch.randint(0, hi, (B,), generator=g).tolist()
