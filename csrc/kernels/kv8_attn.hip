@@ -2,7 +2,7 @@
 //   o = softmax(q k^T scale) v over positions 0 .. pos, queries of a group of heads sharing a key/value head.
 //
 // Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
-// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 49 us, of which the merge 4; a linear read of as much takes 45.
+// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 48 us, of which the merge 4; a linear read of as much takes 45.
 //
 //   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
 // by v_mfma_f32_16x16x32_bf16 on codes that become bf16 in registers, where they are exact, the units' (16 positions) powers of
@@ -19,7 +19,7 @@
 //   a lane's rows straight to registers, kept in the caches    32 x 100 .. 2000 of 128 19.6 / 16.6, 8 x 16384 54.9 / 54.6
 //   the same, not kept (rows of half a line: 40 x 1000 .. 4000 of 64 18.2 -> 19.7)      20.6 / 20.0,            49.8 / 49.3
 //   whole rows by LDS, not kept                                                        18.2 / 17.4,            49.8 / 48.9
-//   and the next tile on its way                                                       16.1 / 15.4,            49.0 / 48.3
+//   and the next tile on its way                                                       16.1 / 15.4,            47.8 / 47.3
 // and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 66.7 cold, 6.1 TB/s; one of 700 keys does not mind.  (Keys of the tile after
 // next asked for as soon as a tile's are read, values alike, was 2 to 8 % slower.)
 //
@@ -235,10 +235,20 @@ struct Kv8State {  // of one wave
 __device__ __forceinline__ int kv8_len(int pos, int slot, const Kv8Pages& pg, int cap) {
   return (unsigned)slot < (unsigned)pg.slots ? min(max(pos, -1), cap - 1) + 1 : 0;
 }
-// units that a row of `len` keys is dealt as: its own and kPad for what a workgroup spends on a row beside its keys
-constexpr int kPad = 6, kLeast = 8;
-__device__ __forceinline__ int kv8_dealt(int len) { return len ? (len + kUnit - 1) / kUnit + kPad : 0; }
+__device__ __forceinline__ int kv8_units(int len) { return (len + kUnit - 1) / kUnit; }
+// Units that a row is dealt as: its own and `pad` for what a workgroup spends on a row beside its keys (48 KB of them), none where no
+// workgroup has parts of two rows (B up to 64: a lane has a row's units), so that shares that are whole turns of the waves stay
+// so.  Us with 6 always, with 6 / 12 / 24 / 48 where rows meet: 1 row (8 heads of 128) of 4,096 keys 10.2, 9.5 all; 2 of 4,096 11.2, 10.4; 8 of
+// 16,384 49.7, 47.6;  4 of 20000 .. 30000 39.1, 39.4 / 39.7 / 40.1 / 40.2;  8 of 64 of 4000 .. 8192 17.8, 18.1 / 17.6 / 17.3 / 16.7;  32 of 2 heads of 32 of
+// 4096 .. 8192 13.1, 13.8 / 13.4 / 13.2 / 12.5.
+constexpr int kLeast = 8;
+constexpr int kv8_pads(int D) { return 48 * 32 / D; }
+__device__ __forceinline__ int kv8_dealt(int units, int pad) { return units ? units + pad : 0; }
 __device__ __forceinline__ int kv8_share(int total, int W) { return max((total + W - 1) / W, kLeast); }
+template <int D>
+__device__ __forceinline__ int kv8_pad(int units, int B, int W) {
+  return B > 64 || (B > 1 && __ballot(units % kv8_share(wave_sum(units), W))) ? kv8_pads(D) : 0;
+}
 
 // EVEN: grid (W, Hkv), shares of all rows' units; else (Hkv, B), a workgroup a row.
 template <int D, int WAVES, bool EVEN>
@@ -260,16 +270,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const int c = lane & 15, g = lane >> 4, rep = Hq / pg.Hkv;
   const int hk = EVEN ? blockIdx.y : blockIdx.x;
   int b = EVEN ? 0 : blockIdx.y, start = 0, from_unit = 0, end = 0, share = 1;
-  int i0 = 0, lens = 0, at_slot = 0;  // EVEN: lane i has row i0 + i
+  int i0 = 0, lens = 0, at_slot = 0, pad = 0;  // EVEN: lane i has row i0 + i
   const auto window = [&](int from) {
     i0 = from;
     at_slot = from + lane < B ? (slots ? slots[from + lane] : from + lane) : -1;
     lens = from + lane < B ? kv8_len(pos[from + lane], at_slot, pg, cap) : 0;
-    return kv8_dealt(lens);
+    return kv8_dealt(kv8_units(lens), pad);
   };
   if constexpr (EVEN) {
-    int total = 0, mine = 0;
-    for (int f = 64 * ((B - 1) / 64); f >= 0; f -= 64) total += mine = window(f);  // (the first rows stay)
+    int total = 0, mine = window(0);
+    pad = __builtin_amdgcn_readfirstlane(kv8_pad<D>(mine, B, gridDim.x));
+    for (int f = 64 * ((B - 1) / 64); f > 0; f -= 64) total += window(f);
+    total += mine = B > 64 ? window(0) : kv8_dealt(mine, pad);  // (the first rows stay)
     total = __builtin_amdgcn_readfirstlane(wave_sum(total));
     share = kv8_share(total, gridDim.x);
     from_unit = blockIdx.x * share;
@@ -294,18 +306,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       if (b - i0 >= 64) window(i0 + 64);
       len = __builtin_amdgcn_readlane(lens, b - i0);
       slot = __builtin_amdgcn_readlane(at_slot, b - i0);
-      n = (len + kUnit - 1) / kUnit;
+      n = kv8_units(len);
       if (n == 0) {  // (units are left, so a later row has them)
         ++b;
         continue;
       }
-      from = start + kPad;  // of its keys
+      from = start + pad;  // of its keys
       u0 = max(from_unit - from, 0), u1 = min(end - from, n);
       if (u1 <= 0) return;  // its keys begin in the next share
     } else {
       slot = slots ? slots[b] : b;
       len = kv8_len(pos[b], slot, pg, cap);
-      n = u1 = (len + kUnit - 1) / kUnit;
+      n = u1 = kv8_units(len);
     }
     u16x8 qf[KS];
     const uint16_t* qrow = q + ((int64_t)b * Hq + hk * rep + min(c, rep - 1)) * D;
@@ -408,16 +420,16 @@ __global__ void __launch_bounds__(C* G)
   float ahead[AHEAD];
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) ahead[i] = po[(int64_t)min(grp + i * G, nparts - 1) * D];
-  const auto len = [&](int i) { return kv8_len(pos[i], slots ? slots[i] : i, pg, cap); };
-  const int n = (len(b) + kUnit - 1) / kUnit;
-  int total = 0, start = 0;
-  for (int i = lane; i < B; i += 64) {
-    const int u = kv8_dealt(len(i));
+  const auto units = [&](int i) { return kv8_units(kv8_len(pos[i], slots ? slots[i] : i, pg, cap)); };
+  const int n = units(b), mine = lane < B ? units(lane) : 0, pad = kv8_pad<D>(mine, B, W);
+  int total = kv8_dealt(mine, pad), start = lane < b ? total : 0;
+  for (int i = lane + 64; i < B; i += 64) {
+    const int u = kv8_dealt(units(i), pad);
     total += u;
     if (i < b) start += u;
   }
   total = wave_sum(total), start = wave_sum(start);
-  const int share = kv8_share(total, W), from = start + kPad;
+  const int share = kv8_share(total, W), from = start + pad;
   const int parts = n > 0 ? (from + n - 1) / share - from / share + 1 : 0;
   if (parts == 1) return;  // written by its workgroup
   float M = -INFINITY, L = 0.f, acc = 0.f;
@@ -465,8 +477,8 @@ using namespace mx;
 // Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB (a CU's 60 GB/s,
 // however many waves); cutting costs a merge and more ends, 2 to 7 us.  Rows that leave no CU alone are better off by four
 // waves, where a CU has the next row's workgroup beside this one's end.  Us, cold, with whole rows of 4 / 8 waves, and cut:
-//   heads of 128: 8 rows of 700 keys 7.5 / 7.2, 8.3; of 1,024 8.7 / 8.6, 8.4; of 2,048 13.4 / 13.2, 8.9;  32 of 1,500 11.4 / 11.5, 11.1;
-//     64 of 1000 .. 2000 13.7 / 13.9, 14.4; of 16,384 88.9 / 84.8, 49.5;  128 of 1000 .. 2000 14.6 / 15.1, 19.2; of 2000 .. 4096 24.8 / 25.6,
+//   heads of 128: 8 rows of 700 keys 7.5 / 7.2, 8.3; of 1,024 8.7 / 8.6, 8.3; of 2,048 13.4 / 13.2, 8.3;  32 of 1,500 11.4 / 11.5, 11.1;
+//     64 of 1000 .. 2000 13.7 / 13.9, 14.4; of 16,384 88.9 / 84.8, 47.8;  128 of 1000 .. 2000 14.6 / 15.1, 19.2; of 2000 .. 4096 24.8 / 25.6,
 //     26.1;  192 of 100 .. 4096 25.5 / 26.6, 27.2;  256 of 100 .. 2000 16.0 / 16.8, 21.3; of 100 .. 4096 27.4 / 28.4, 33.6;  512 of 30 .. 512
 //     10.6 / 12.8, 20.0; of 2048 .. 4096 66.8 / 70.1, 72.2
 //   of 64: 8 of 700 6.1 / 5.4, 7.5; of 2,048 11.3 / 8.9, 8.1;  64 of 1000 .. 3000 14.6 / 10.9, 12.4;  128 of 500 .. 2000 11.5 / 9.1, 13.9; of 1000
@@ -542,7 +554,7 @@ extern "C" int mx_kv8_attn(const uint16_t* q, const Kv8Pages* cache, const int32
   if (B <= 0) return 0;
   const Kv8Pages pg = *cache;
   if (pg.Hkv <= 0 || Hq % pg.Hkv || Hq / pg.Hkv > 16 || B > 65535 || pg.Hkv > 65535 || cap < 1 ||
-      (int64_t)B * (cap / kUnit + 1 + kPad) > INT32_MAX || (int64_t)B * Hq * (D / 32) > INT32_MAX || !(scale > 0.f))
+      (int64_t)B * (cap / kUnit + 1 + kv8_pads(D)) > INT32_MAX || (int64_t)B * Hq * (D / 32) > INT32_MAX || !(scale > 0.f))
     return -1;
   const Launch a{q, pg, pos, slots, part_ml, part_o, out, B, Hq, cap, scale * 1.4426950408889634f, stream};
   if (D == 128) launch<128>(a);

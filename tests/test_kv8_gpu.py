@@ -214,7 +214,8 @@ def test_attention_of_short_rows(gpu, D, Hq, Hkv, block):
     _check_attention(gpu, [0, 1, 15, 16, 17, 31, 33, 63, 65, 128, 255, 256, 257, 511, 512], Hq, Hkv, block, D)
 
 
-@pytest.mark.parametrize("lens", [[513], [1, 4000, 0, 17, 700], [2048] * 9, [0, 0, 1000], [30000, 1, 16], list(range(1, 900, 13))])
+@pytest.mark.parametrize("lens", [[513], [1, 4000, 0, 17, 700], [2048] * 9, [0, 0, 1000], [30000, 1, 16], list(range(1, 900, 13)), [4096] * 2,
+                                  [4500, *range(1, 900, 13)], [5000, 0, 3000, *range(0, 260, 2)]])
 @pytest.mark.parametrize("D,Hq,Hkv", HEADS[:4])
 def test_attention_of_long_and_uneven_rows(gpu, D, Hq, Hkv, lens):
     _check_attention(gpu, lens, Hq, Hkv, 256, D, seed=len(lens))
