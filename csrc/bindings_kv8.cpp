@@ -3,6 +3,7 @@
 #include "bindings_util.h"
 #include "kernels/kv8_pages.h"
 
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -148,16 +149,29 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor
   return {dqkv, dwq, dwk};
 }
 
+// The ops for autograd's kernel, which calls them through the dispatcher: whatever records, batches or stands in for calls
+// (tracers, dispatch modes, batches of backwards) then meets the op and not the allocations inside it.
+const auto& forward_op() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("mxllm::qk_norm_rope", "").typed<decltype(qk_norm_rope)>();
+  return op;
+}
+const auto& backward_op() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("mxllm::qk_norm_rope_bwd", "").typed<decltype(qk_norm_rope_bwd)>();
+  return op;
+}
+
 // The same for autograd, here as its Python form (mxllm/ops/attention.py, which a weight with an owner takes) costs 40 us of the host's
-// time a step more, as much as 2,048 rows of 48 heads of 128 take forward and backward.
+// time a step more, as much as 2,048 rows of 48 heads of 128 take forward and backward.  (Rows that the kernels cannot read as
+// they lie are copied by either op: only below the dispatcher is there an address to look at.)
 struct QKNormRope : torch::autograd::Function<QKNormRope> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& any,
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv,
                                                 const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& cos,
                                                 const at::Tensor& sin, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                 double eps, const OptTensor& positions) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor qkv = rows16(any);
-    auto [q, k, v] = qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
+    auto [q, k, v] = forward_op().call(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
     ctx->save_for_backward({qkv, wq, wk, cos, sin, given(positions) ? *positions : at::Tensor()});
     ctx->saved_data["Hkv"] = Hkv;
     ctx->saved_data["eps"] = eps;
@@ -171,10 +185,10 @@ struct QKNormRope : torch::autograd::Function<QKNormRope> {
     torch::autograd::variable_list out(12);
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dqkv, dwq, dwk] = qk_norm_rope_bwd(g[0].contiguous(), g[1].contiguous(), g[2].contiguous(), saved[0], saved[1],
-                                               saved[2], saved[3], saved[4], ctx->saved_data["Hkv"].toInt(),
-                                               ctx->saved_data["eps"].toDouble(),
-                                               saved[5].defined() ? OptTensor(saved[5]) : c10::nullopt, 0, need_q || need_k, false);
+      auto [dqkv, dwq, dwk] = backward_op().call(
+          g[0].contiguous(), g[1].contiguous(), g[2].contiguous(), saved[0], saved[1], saved[2], saved[3], saved[4],
+          ctx->saved_data["Hkv"].toInt(), ctx->saved_data["eps"].toDouble(),
+          saved[5].defined() ? OptTensor(saved[5]) : c10::nullopt, 0, need_q || need_k, false);
       out[0] = dqkv;
       if (need_q) out[1] = dwq;
       if (need_k) out[2] = dwk;
@@ -201,7 +215,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_grad(const at::Tenso
     recorded = recorded || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
   if (!recorded) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
+    return forward_op().call(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, positions);
   }
   if (at::GradMode::is_enabled()) {
     DevGuard g(qkv.device());
