@@ -27,6 +27,9 @@
 // shares, one a workgroup of a KV head, whose waves share what it has of a sequence, and sequences that were cut are merged by a
 // second launch.  Where a row is cut follows from the lengths of all, so the last bits of an output may
 // differ from batch to batch (the same call has the same bits).
+//
+// Waves and parts hand on means, sum of w v over sum of w, which are no larger than the values are; a wave's own sums, of weights up
+// to 2^8, are held in units of 2^32 as soon as a unit of its keys has values that could take them past the end of f32 (kFar).
 #include "kv8.h"
 
 namespace mx {
@@ -37,6 +40,9 @@ typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(1))) const void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 constexpr int kNt = 2;  // of a load: read once
+// The exponent byte of values from which on a wave's sums are in units of 2^32: below it 2^21 weights of 2^8 of values up to
+// 448 * 2^80 stay under 2^127.  (Beside values of 2^81 and more those under 2^-86 count for up to that much.)
+constexpr int kFar = 208, kFarBy = 32;
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4v& a, const u16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
@@ -69,9 +75,10 @@ struct Kv8State {  // of one wave
   static constexpr int E = D / 16, KS = D / 32;
   float m, l;   // reference of the exponents of head c; l: this lane's keys
   f32x4 o[E];   // [e][i]: channel E (4 g + i) + e of head c
+  bool far;     // o is in units of 2^kFarBy (the same in all lanes)
 
   __device__ __forceinline__ void clear() {
-    m = -INFINITY, l = 0.f;
+    m = -INFINITY, l = 0.f, far = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -231,6 +238,10 @@ struct Kv8State {  // of one wave
   }
 };
 
+// a row's output: zero without keys; keys that all score -inf have no softmax
+__device__ __forceinline__ float kv8_output(float mean, float sum, int units) {
+  return units == 0 ? 0.f : sum == 0.f ? __builtin_nanf("") : mean;
+}
 // keys of a row: none where its slot is none of the table's
 __device__ __forceinline__ int kv8_len(int pos, int slot, const Kv8Pages& pg, int cap) {
   return (unsigned)slot < (unsigned)pg.slots ? min(max(pos, -1), cap - 1) + 1 : 0;
@@ -337,7 +348,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const int64_t unit = kv8_unit(pg, slot, min(mine, u1 - 1), hk);
       const int where = (int)max(unit, (int64_t)0);
       const float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)pg.ke[where] << 23);
-      const float vs = __uint_as_float((uint32_t)pg.ve[where] << 23);
+      int ve = pg.ve[where];
       const int tiles = min(32, (u1 - t0 + 2 * WAVES - 1) / (2 * WAVES));  // of this wave, here
       const int whole = min(u1, len / kUnit);                                // units before this one have all their rows
       const auto fetch = [&](int i, int half) {
@@ -351,6 +362,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
       constexpr int LOADS = D / 16;  // of a tile
       fetch(0, 0);
+      if (!st.far && __ballot(ve >= kFar)) {  // (behind the first fetch, which does not wait for exponents)
+        st.far = true;
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.o[e] *= 0x1p-32f;
+      }
+      if (st.far) ve = max(ve - kFarBy, 1);
+      const float vs = __uint_as_float((uint32_t)ve << 23);
       for (int i = 0; i < tiles; ++i) {
         if (i + 1 < tiles) {
           fetch(i + 1, (i + 1) & 1);
@@ -364,11 +382,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       }
     }
     st.l = lane_sum<32>(lane_sum<16>(st.l));
+    const float inv = st.l == 0.f ? 1.f : __builtin_amdgcn_rcpf(st.l), up = st.far ? 0x1p32f : 1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       orow_t y;
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = st.o[e][i];
+      for (int e = 0; e < E; ++e) y[e] = st.o[e][i] * inv * up;
       *reinterpret_cast<orow_t*>(reinterpret_cast<float*>(smem + w * PART) + c * ROW + E * (4 * g + i)) = y;
     }
     if (g == 0) mls[w][0][c] = st.m, mls[w][1][c] = st.l;
@@ -376,18 +395,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
     const int part = EVEN ? (int)blockIdx.x - from / share : 0, last = EVEN ? (from + n - 1) / share - from / share : 0;
     for (int idx = tid; idx < rep * D; idx += 64 * WAVES) {
       const int h = idx / D, d = idx % D;
-      float M = -INFINITY, L = 0.f, acc = 0.f;
+      float M = -INFINITY, L = 0.f, acc = 0.f, f[WAVES];
 #pragma unroll
       for (int x = 0; x < WAVES; ++x) M = fmaxf(M, mls[x][0][h]);
 #pragma unroll
       for (int x = 0; x < WAVES; ++x) {  // (a wave whose scores are NaN has no maximum, and its sum carries them)
-        const float mw = mls[x][0][h], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-        L += f * mls[x][1][h];
-        acc += f * reinterpret_cast<const float*>(smem + x * PART)[h * ROW + d];
+        const float mw = mls[x][0][h];
+        f[x] = (mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M)) * mls[x][1][h];
+        L += f[x];
       }
+      const float all = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L);
+#pragma unroll
+      for (int x = 0; x < WAVES; ++x) acc += f[x] * all * reinterpret_cast<const float*>(smem + x * PART)[h * ROW + d];
       const int64_t bh = (int64_t)b * Hq + hk * rep + h;
-      if (last == 0) {  // the row's only part is its output (keys that all score -inf leave 0 / 0)
-        out[bh * D + d] = f2bf(n ? acc / L : 0.f);
+      if (last == 0) {  // the row's only part is its output
+        out[bh * D + d] = f2bf(kv8_output(acc, L, n));
       } else {
         part_o[(bh * nparts + part) * D + d] = acc;
         if (d == 0) part_ml[(bh * nparts + part) * 2] = M, part_ml[(bh * nparts + part) * 2 + 1] = L;
@@ -438,11 +460,13 @@ __global__ void __launch_bounds__(C* G)
     const float2 x = p0 ? ml[min(p0 + lane, nparts - 1)] : first;
     const float m = on ? x.x : -INFINITY, top = fmaxf(M, wave_max(m));
     const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    L = L * was + wave_sum(on ? f * x.y : 0.f);
-    acc *= was;
+    const float kept = L * was, fl = on ? f * x.y : 0.f;
+    L = kept + wave_sum(fl);
+    const float inv = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L), share_of = fl * inv;
+    acc *= kept * inv;
     M = top;
     const int end = min(64, parts - p0);
-    const auto weight = [&](int s) { return __shfl(f, s); };  // (of this wave's groups)
+    const auto weight = [&](int s) { return __shfl(share_of, s); };  // (of this wave's groups)
     int i = 0;
     if (p0 == 0) {
 #pragma unroll
@@ -467,7 +491,7 @@ __global__ void __launch_bounds__(C* G)
 #pragma unroll
     for (int i = 0; i < G; ++i) acc += sums[i][threadIdx.x];
   }
-  out[bh * D + d] = f2bf(n ? acc / L : 0.f);
+  out[bh * D + d] = f2bf(kv8_output(acc, L, n));
 }
 
 }  // namespace mx
