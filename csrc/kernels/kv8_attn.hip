@@ -70,15 +70,42 @@ __device__ __forceinline__ int chan(int s, int g) {
   return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
 }
 
+// Products of queries and codes come ahead of the codes' power of two, so the queries of a head (that of four lanes) that could
+// take their sum past f32 are divided by 2^qe = 2^32 (else 1); true: some head's are.  128 products of 2^96 and codes up to 448
+// stay under 2^112.
+template <int KS>
+__device__ __forceinline__ bool shrink_queries(u16x8 (&q)[KS], int& qe) {
+  constexpr uint16_t kBig = (127 + 96) << 7;
+  uint16_t top = 0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, (uint16_t)(q[s][j] & 0x7fff));
+  }
+  qe = 0;
+  if (!__ballot(top >= kBig)) return false;
+  if (lane_max<32>(lane_max<16>(bf2f(top))) >= 0x1p96f) {
+    qe = 32;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[s][j] = f2bf(bf2f(q[s][j]) * 0x1p-32f);
+    }
+  }
+  return true;
+}
+
 template <int D>
 struct Kv8State {  // of one wave
   static constexpr int E = D / 16, KS = D / 32;
   float m, l;   // reference of the exponents of head c; l: this lane's keys
   f32x4 o[E];   // [e][i]: channel E (4 g + i) + e of head c
+  int qe;       // the power of two that the queries of head c were divided by
+  bool big;     // some head's were (the same in all lanes)
   bool far;     // o is in units of 2^kFarBy (the same in all lanes)
 
   __device__ __forceinline__ void clear() {
-    m = -INFINITY, l = 0.f, far = false;
+    m = -INFINITY, l = 0.f, qe = 0, big = far = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -144,10 +171,10 @@ struct Kv8State {  // of one wave
     }
   }
 
-  // off: the tile's half; ks: what the units' scores are multiplied by, vs: powers of two of their values; all: every row is
-  // there, else up to lim0, lim1
+  // off: the tile's half; ks: what the units' scores are multiplied by (NaN: the units are none), where `big` the powers of two
+  // beside sl; vs: powers of two of their values; all: every row is there, else up to lim0, lim1
   __device__ __forceinline__ void take(const Places& from, uint32_t off, const u16x8 (&qf)[KS], float ks0, float ks1,
-                                       float vs0, float vs1, bool all, int lim0, int lim1, int c, int g) {
+                                       float vs0, float vs1, float sl, bool all, int lim0, int lim1, int c, int g) {
     Places at = from;
 #pragma unroll
     for (uint32_t& x : at.k) x += off;
@@ -198,6 +225,13 @@ struct Kv8State {  // of one wave
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * (i < 4 ? ks0 : ks1);
+    if (big) {  // ks is small, down to where f32 has few bits, where queries are so large: powers of two by themselves
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float k = i < 4 ? ks0 : ks1;
+        x[i] = k == k ? __builtin_ldexpf(sc[i >> 2][i & 3] * sl, (int)k + qe) : k;
+      }
+    }
     if (!all) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = 4 * g + (i & 3) <= (i < 4 ? lim0 : lim1) ? x[i] : -INFINITY;
@@ -347,7 +381,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const int mine = t0 + 2 * WAVES * (lane >> 1) + (lane & 1);
       const int64_t unit = kv8_unit(pg, slot, min(mine, u1 - 1), hk);
       const int where = (int)max(unit, (int64_t)0);
-      const float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)pg.ke[where] << 23);
+      const int ke = pg.ke[where];
+      float ks = unit < 0 ? __builtin_nanf("") : sl * __uint_as_float((uint32_t)ke << 23);
       int ve = pg.ve[where];
       const int tiles = min(32, (u1 - t0 + 2 * WAVES - 1) / (2 * WAVES));  // of this wave, here
       const int whole = min(u1, len / kUnit);                                // units before this one have all their rows
@@ -362,7 +397,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const auto of = [](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
       constexpr int LOADS = D / 16;  // of a tile
       fetch(0, 0);
-      if (!st.far && __ballot(ve >= kFar)) {  // (behind the first fetch, which does not wait for exponents)
+      // (behind the first fetch, which waits neither for queries nor for exponents)
+      if (t0 == u0 + 2 * w) st.big = shrink_queries<KS>(qf, st.qe);
+      if (st.big && unit >= 0) ks = (float)(ke - 127);
+      if (!st.far && __ballot(ve >= kFar)) {
         st.far = true;
 #pragma unroll
         for (int e = 0; e < E; ++e) st.o[e] *= 0x1p-32f;
@@ -377,8 +415,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
           __builtin_amdgcn_s_waitcnt(0x0F70);
         }
         const int u = t0 + 2 * WAVES * i, lim = len - 1 - kUnit * u, lim1 = u + 1 < u1 ? lim - kUnit : -1;
-        st.take(at, (i & 1) * (64 * D), qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), u + 2 <= whole,
-                lim, lim1, c, g);
+        st.take(at, (i & 1) * (64 * D), qf, of(ks, 2 * i), of(ks, 2 * i + 1), of(vs, 2 * i), of(vs, 2 * i + 1), sl,
+                u + 2 <= whole, lim, lim1, c, g);
       }
     }
     st.l = lane_sum<32>(lane_sum<16>(st.l));

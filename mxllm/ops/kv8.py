@@ -174,8 +174,7 @@ def decode_attention(q: torch.Tensor, pages: Pages, pos: torch.Tensor, slots: to
                      scale: float | None = None) -> torch.Tensor:
     """One token of each sequence: q [B, Hq, D] over positions 0 .. pos[b] of slot slots[b] (int32 [B]; None: the rows'
     numbers) -> [B, Hq * D].  ``max_len`` >= 1 bounds the positions that any row looks at (a host number, for the launch;
-    positions at it and behind are not seen), ``scale`` > 0.  A row without keys (pos < 0, or a slot that is none) gives zeros.
-    The GPU multiplies queries with codes ahead of their power of two: queries of 2 ** 111 and more may overflow."""
+    positions at it and behind are not seen), ``scale`` > 0.  A row without keys (pos < 0, or a slot that is none) gives zeros."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if use_native(q):
         return native().kv8_decode_attn(q, *pages, pos, slots, max_len, scale)
