@@ -233,7 +233,7 @@ mx::Kv8Pages check_pages(const at::Tensor& k, const at::Tensor& v, const at::Ten
     MX_CHECK(t.device() == like.device() && t.scalar_type() == at::kByte && t.is_contiguous(),
              "8-bit cache: contiguous uint8 tensors on the device of the rows");
   }
-  MX_CHECK(k.dim() == 4 && k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 16 && k.size(2) % 16 == 0 &&
+  MX_CHECK(k.dim() == 4 && k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 16 && k.size(2) % 16 == 0 && k.size(3) >= 1 &&
                v.sizes() == k.sizes(),
            "8-bit cache: codes [pages, Hkv, block, D] with blocks of a multiple of 16 positions, got ", k.sizes(), " and ",
            v.sizes());

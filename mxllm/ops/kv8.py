@@ -212,7 +212,7 @@ def _check_pages(pages: Pages) -> None:
     k, v, ke, ve, table = pages
     want = (*k.shape[:2], k.shape[2] // GROUP) if k.dim() == 4 else None
     if (any(t.dtype != torch.uint8 for t in (k, v, ke, ve)) or k.dim() != 4 or v.shape != k.shape or k.shape[2] % GROUP
-            or k.shape[2] == 0 or tuple(ke.shape) != want or tuple(ve.shape) != want):
+            or 0 in k.shape or tuple(ke.shape) != want or tuple(ve.shape) != want):
         raise ValueError("8-bit cache: uint8 codes [pages, Hkv, block, D] (block a multiple of 16), exponents [pages, Hkv, block / 16]")
     if table.dtype != torch.int32 or table.dim() != 2:
         raise ValueError("block table: int32 [slots, max_pages]")
