@@ -357,10 +357,14 @@ at::Tensor kv8_decode_attn(const at::Tensor& q_any, const at::Tensor& kc, const 
   return out;
 }
 
-// causal attention inside each segment of blocks [n, 4] (mxllm/ops/hybrid.py PromptRows.attn_blocks): q [Hq, T, D], k, v
-// [Hkv, T, D] -> [T, Hq * D]
-at::Tensor prompt_rows_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& blocks,
-                                 double scale) {
+// causal attention inside each segment of blocks [n, 4] (mxllm/ops/hybrid.py PromptRows.attn_blocks), which name every row: q
+// [Hq, T, D], k, v [Hkv, T, D] -> [T, Hq * D]
+at::Tensor prompt_rows_attention(const at::Tensor& q_any, const at::Tensor& k_any, const at::Tensor& v_any,
+                                 const at::Tensor& blocks_any, double scale) {
+  MX_CHECK(q_any.is_cuda(), "q: on the GPU");
+  DevGuard g(q_any.device());
+  const at::Tensor q = placed(q_any.contiguous()), k = placed(k_any.contiguous()), v = placed(v_any.contiguous()),
+                   blocks = placed(blocks_any);
   check_bf16(q, "q");
   check_bf16(k, "k");
   check_bf16(v, "v");
@@ -372,7 +376,6 @@ at::Tensor prompt_rows_attention(const at::Tensor& q, const at::Tensor& k, const
   MX_CHECK(T * D * 2 < INT32_MAX, "prompt_rows_attention: too many rows");
   MX_CHECK(blocks.dim() == 2, "blocks int32 [n, 4]");
   const int32_t* bl = check_ints(blocks, {blocks.size(0), 4}, q, "blocks");
-  DevGuard g(q.device());
   auto o = at::empty({T, Hq * D}, q.options());
   const int rc = mx_attn_fwd_prompts(bf(q), bf(k), bf(v), bl, (int)blocks.size(0), bfm(o), (int)T, (int)Hq, (int)Hkv, (int)D,
                                      (float)scale, cur_stream());

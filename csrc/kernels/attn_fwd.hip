@@ -130,6 +130,7 @@ attn_fwd_kernel(const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K, 
   size_t qo = (size_t)(b * Hq + h) * S, ko = (size_t)(b * Hkv + hk) * Sk;
   if constexpr (SEG) {
     const int4 sg = seg.blocks[bid / BH];
+    if (sg.x < 0 || sg.y < 1 || sg.x > seg.T - sg.y || sg.z < 0 || sg.z > (sg.y - 1) / BM) return;  // a block of no rows here
     row0 = sg.x, S = sg.y, Sk = sg.y, qb = sg.z;
     qo = (size_t)h * seg.T + row0, ko = (size_t)hk * seg.T + row0;
   }

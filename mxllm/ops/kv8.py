@@ -22,6 +22,7 @@ import torch
 
 from . import reference as ref
 from ._ext import native, use_native
+from .hybrid import PromptRows
 
 GROUP = 16  # positions that share an exponent
 E4M3 = torch.float8_e4m3fn
@@ -139,16 +140,25 @@ def append_prompts(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, runs
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: list[int],
                      blocks: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of each of several prompts to itself: q [Hq, T, D], k, v [Hkv, T, D] of sequences of ``lens`` rows one
-    after another (``append_prompts`` from position 0) -> [T, Hq * D].  ``blocks``: the table of 128-row blocks
-    (``PromptRows.attn_blocks(max(lens))``), which the GPU needs."""
+    after another, T in all (``append_prompts`` from position 0) -> [T, Hq * D].  ``blocks``: the table of 128-row blocks that the
+    GPU takes, made here (and sent there) if it is not given; for many layers it is made once:
+    ``PromptRows(lens, device).attn_blocks(max(lens))``."""
+    if q.dim() != 3 or k.dim() != 3 or sum(lens) != q.shape[1] or any(n < 0 for n in lens):
+        raise ValueError(f"lens of q's rows, got {lens} of {list(q.shape)}")
     if use_native(q):
+        if blocks is None:
+            blocks = PromptRows([n for n in lens if n], q.device).attn_blocks(max(lens)) if sum(lens) else q.new_zeros(0, 4).int()
+        if blocks.shape[0] != sum(-(-n // 128) for n in lens):
+            raise ValueError(f"blocks of 128 rows of {lens}, got {blocks.shape[0]}")
         return native().prompt_rows_attention(q, k, v, blocks, 1.0 / math.sqrt(q.shape[-1]))
-    out, at = [], 0
+    if q.shape[0] % max(k.shape[0], 1) or k.shape[0] == 0 or k.shape[1:] != q.shape[1:] or v.shape != k.shape:
+        raise ValueError(f"q [Hq, T, D], k, v [Hkv, T, D], got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    out, at = q.new_empty(q.shape[1], q.shape[0] * q.shape[2]), 0
     for n in lens:
         o = ref.attention(*(x[None, :, at:at + n].transpose(1, 2) for x in (q, k, v)))
-        out.append(o.reshape(n, -1))
+        out[at:at + n] = o.flatten(2)[0]
         at += n
-    return torch.cat(out)
+    return out
 
 
 def read(pages: Pages, slots: torch.Tensor | None, starts: torch.Tensor, ends: torch.Tensor, n: int):
