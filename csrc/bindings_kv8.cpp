@@ -344,11 +344,11 @@ at::Tensor kv8_decode_attn(const at::Tensor& q_any, const at::Tensor& kc, const 
   const int64_t cap = std::min<int64_t>(max_len, (int64_t)pg.maxp * pg.block);
   auto out = at::empty({B, Hq * D}, q.options());
   const int64_t parts = mx_kv8_attn_parts((int)B, (int)Hkv, (int)D, (int)cap);
-  at::Tensor work;  // outputs of the parts [B, Hq, parts, D], then their maxima and sums [B, Hq, parts, 2]
+  at::Tensor work;  // outputs of the parts [Hq, parts, D], then their maxima and sums [Hq, parts, 2]
   float *po = nullptr, *ml = nullptr;
   if (parts) {
-    work = at::empty({B * Hq * parts * (D + 2)}, q.options().dtype(at::kFloat));
-    po = work.data_ptr<float>(), ml = po + B * Hq * parts * D;
+    work = at::empty({Hq * parts * (D + 2)}, q.options().dtype(at::kFloat));
+    po = work.data_ptr<float>(), ml = po + Hq * parts * D;
   }
   const int rc = mx_kv8_attn(bf(q), &pg, p, sl, ml, po, bfm(out), (int)B, (int)Hq, (int)D, (int)cap, (float)scale,
                              cur_stream());

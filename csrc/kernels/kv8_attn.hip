@@ -295,6 +295,11 @@ __device__ __forceinline__ int kv8_pad(int units, int B, int W) {
   return B > 64 || (B > 1 && __ballot(units % kv8_share(wave_sum(units), W))) ? kv8_pads(D) : 0;
 }
 
+// Where workgroup x of W leaves what it has of a row that was cut: it has at most one that began before its share (part > 0) and one
+// that goes on behind it (part 0), so 2 W places a query head hold the parts of any batch.  By row, parts would take B times what
+// one row can be cut into (1,024 rows of up to 32,768 keys of one head of 128, 16 query heads: 2.2 GB for 4 MB).
+__device__ __forceinline__ int64_t kv8_place(int head, int x, int part, int W) { return ((int64_t)head * 2 + (part ? 0 : 1)) * W + x; }
+
 // EVEN: grid (W, Hkv), shares of all rows' units; else (Hkv, B), a workgroup a row.
 template <int D, int WAVES, bool EVEN>
 __global__ void __launch_bounds__(64 * WAVES, 2)
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
                     const uint16_t* __restrict__ q, uint8_t* __restrict__ keys, uint8_t* __restrict__ values,
                     uint8_t* __restrict__ key_exps, uint8_t* __restrict__ value_exps, int nslots, int maxp, int block,
                     int pages, int Hkv, float* __restrict__ part_ml, float* __restrict__ part_o,
-                    uint16_t* __restrict__ out, int B, int Hq, int cap, int nparts, float sl) {
+                    uint16_t* __restrict__ out, int B, int Hq, int cap, float sl) {
   const Kv8Pages pg{keys, values, key_exps, value_exps, table, nslots, maxp, block, pages, Hkv};
   typedef Kv8State<D> State;
   constexpr int E = State::E, KS = State::KS, ROW = D + 8;  // (rows of whole pieces of 32 bytes)
@@ -449,8 +454,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       if (last == 0) {  // the row's only part is its output
         out[bh * D + d] = f2bf(kv8_output(acc, L, n));
       } else {
-        part_o[(bh * nparts + part) * D + d] = acc;
-        if (d == 0) part_ml[(bh * nparts + part) * 2] = M, part_ml[(bh * nparts + part) * 2 + 1] = L;
+        const int64_t at = kv8_place(hk * rep + h, blockIdx.x, part, gridDim.x);
+        part_o[at * D + d] = acc;
+        if (d == 0) part_ml[at * 2] = M, part_ml[at * 2 + 1] = L;
       }
     }
     if constexpr (!EVEN) return;
@@ -462,24 +468,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 }
 
 // The parts of rows that were cut, and the zeros of rows without keys; W: workgroups of a KV head.  A workgroup has C channels of a
-// row, and G groups of its threads share the parts; a lane has the maximum and the sum of one of 64 parts.  What comes
-// from memory comes at once: the first parts are loaded (where the buffers have room) before they are known to be any.
+// row, and G groups of its threads share the parts; a lane has the maximum and the sum of one of 64 parts.  Where the parts
+// lie follows from the lengths; what comes from memory after them comes at once.
 template <int D, int C, int G>
 __global__ void __launch_bounds__(C* G)
     kv8_merge_kernel(const float* __restrict__ part_ml, const float* __restrict__ part_o, Kv8Pages pg,
                      const int32_t* __restrict__ pos, const int32_t* __restrict__ slots, uint16_t* __restrict__ out, int B,
-                     int Hq, int W, int cap, int nparts) {
+                     int Hq, int W, int cap) {
   constexpr int AHEAD = G >= 8 ? 2 : G >= 4 ? 3 : 4;
   __shared__ float sums[G][C];
   const int64_t bh = blockIdx.x / (D / C);
-  const int b = (int)(bh / Hq), lane = threadIdx.x & 63, grp = threadIdx.x / C;
+  const int b = (int)(bh / Hq), head = (int)(bh % Hq), lane = threadIdx.x & 63, grp = threadIdx.x / C;
   const int d = C * (blockIdx.x % (D / C)) + threadIdx.x % C;
-  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * nparts;
-  const float* po = part_o + bh * nparts * D + d;
-  const float2 first = ml[min(lane, nparts - 1)];
-  float ahead[AHEAD];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) ahead[i] = po[(int64_t)min(grp + i * G, nparts - 1) * D];
   const auto units = [&](int i) { return kv8_units(kv8_len(pos[i], slots ? slots[i] : i, pg, cap)); };
   const int n = units(b), mine = lane < B ? units(lane) : 0, pad = kv8_pad<D>(mine, B, W);
   int total = kv8_dealt(mine, pad), start = lane < b ? total : 0;
@@ -489,13 +489,22 @@ __global__ void __launch_bounds__(C* G)
     if (i < b) start += u;
   }
   total = wave_sum(total), start = wave_sum(start);
-  const int share = kv8_share(total, W), from = start + pad;
-  const int parts = n > 0 ? (from + n - 1) / share - from / share + 1 : 0;
+  const int share = kv8_share(total, W), from = start + pad, x0 = from / share;
+  const int parts = n > 0 ? (from + n - 1) / share - x0 + 1 : 0;
   if (parts == 1) return;  // written by its workgroup
+  const auto ml = [&](int p) { return reinterpret_cast<const float2*>(part_ml)[kv8_place(head, x0 + p, p, W)]; };
+  const auto po = [&](int p) { return part_o[kv8_place(head, x0 + p, p, W) * D + d]; };
+  float2 first = {0.f, 0.f};
+  float ahead[AHEAD] = {};
+  if (parts) {
+    first = ml(min(lane, parts - 1));
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = po(min(grp + i * G, parts - 1));
+  }
   float M = -INFINITY, L = 0.f, acc = 0.f;
   for (int p0 = 0; p0 < parts; p0 += 64) {
     const bool on = p0 + lane < parts;
-    const float2 x = p0 ? ml[min(p0 + lane, nparts - 1)] : first;
+    const float2 x = p0 ? ml(min(p0 + lane, parts - 1)) : first;
     const float m = on ? x.x : -INFINITY, top = fmaxf(M, wave_max(m));
     const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
     const float kept = L * was, fl = on ? f * x.y : 0.f;
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(C* G)
 #pragma unroll 8
     for (; i * G < end; ++i) {  // (every lane takes the same turns)
       const int s = grp + i * G;
-      const float wgt = weight(min(s, 63)), y = po[(int64_t)(p0 + min(s, end - 1)) * D];
+      const float wgt = weight(min(s, 63)), y = po(p0 + min(s, end - 1));
       if (s < end) acc += wgt * y;
     }
   }
@@ -558,11 +567,9 @@ static int kv8_waves(int64_t rows, int64_t cap, int D) {
 // 18.1;  64 of 32 of 4096 .. 8192 13.7, 13.1, 14.4.  (768 of four waves 23.8 and 55.0 where 512 have 20.2 and 49.3.)
 static int kv8_shares(int Hkv) { return Hkv < 256 ? (256 + Hkv - 1) / Hkv : 1; }
 
-// parts that a row of up to `cap` keys can be cut into (of part_ml [B, Hq, parts, 2], part_o [B, Hq, parts, D]); 0: rows are whole
+// places for parts that a query head has (of part_ml [Hq, places, 2], part_o [Hq, places, D]); 0: rows are whole
 extern "C" int mx_kv8_attn_parts(int B, int Hkv, int D, int cap) {
-  if (kv8_waves((int64_t)B * Hkv, cap, D)) return 0;
-  const int W = kv8_shares(Hkv), most = (cap / kUnit + 1) / kLeast + 2;
-  return W < most ? W : most;
+  return kv8_waves((int64_t)B * Hkv, cap, D) ? 0 : 2 * kv8_shares(Hkv);
 }
 
 namespace {
@@ -582,14 +589,13 @@ template <int D, int WAVES>
 void launch_whole(const Launch& a) {
   kv8_attn_kernel<D, WAVES, false><<<dim3(a.pg.Hkv, a.B), 64 * WAVES, 0, a.stream>>>(
       a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages,
-      a.pg.Hkv, nullptr, nullptr, a.out, a.B, a.Hq, a.cap, 0, a.sl);
+      a.pg.Hkv, nullptr, nullptr, a.out, a.B, a.Hq, a.cap, a.sl);
 }
 
 template <int D>
 void launch(const Launch& a) {
-  const int Hkv = a.pg.Hkv, nparts = mx_kv8_attn_parts(a.B, Hkv, D, a.cap), W = kv8_shares(Hkv);
-  if (!nparts) {
-    const int waves = kv8_waves((int64_t)a.B * Hkv, a.cap, D);
+  const int Hkv = a.pg.Hkv, W = kv8_shares(Hkv), waves = kv8_waves((int64_t)a.B * Hkv, a.cap, D);
+  if (waves) {
     if (waves == 4) launch_whole<D, 4>(a);
     else launch_whole<D, 8>(a);
     return;
@@ -597,14 +603,14 @@ void launch(const Launch& a) {
   constexpr int WAVES = D == 128 ? 4 : 8;
   kv8_attn_kernel<D, WAVES, true><<<dim3(W, Hkv), 64 * WAVES, 0, a.stream>>>(
       a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages, Hkv,
-      a.part_ml, a.part_o, a.out, a.B, a.Hq, a.cap, nparts, a.sl);
+      a.part_ml, a.part_o, a.out, a.B, a.Hq, a.cap, a.sl);
   const int rows = a.B * a.Hq;
   if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.5 -> 10.8 us, 1 x 32768 34.1 -> 20.3
     kv8_merge_kernel<D, 32, 8><<<rows * (D / 32), 256, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots, a.out, a.B,
-                                                                      a.Hq, W, a.cap, nparts);
+                                                                      a.Hq, W, a.cap);
   else
     kv8_merge_kernel<D, D, D < 128 ? 128 / D : 1><<<rows, 128, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots,
-                                                                              a.out, a.B, a.Hq, W, a.cap, nparts);
+                                                                              a.out, a.B, a.Hq, W, a.cap);
 }
 
 }  // namespace
