@@ -151,6 +151,9 @@ def _norm_grads(ctx, dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, gra
     dqkv, *dws = native().qk_norm_rope_bwd(dq, dk, dv, qkv, wq, wk, cos, sin, Hkv, eps, positions, grad_pad, any(need),
                                            any(owned))
     out = [None, None]
+    if owned[0] and ctx.leaves[0] is ctx.leaves[1]:  # one weight for both norms: its owner hears of it once, with the sum
+        if accum_grad(ctx.leaves[0], dws[0] + dws[1]):
+            return dqkv, *out
     for i, (leaf, dw) in enumerate(zip(ctx.leaves, dws)):
         if need[i] and not (owned[i] and accum_grad(leaf, dw)):
             out[i] = dw.to(wq.dtype)
