@@ -1,11 +1,14 @@
-"""``attention_block(norms=)`` and ``qk_norm_rope``: their weights' gradients where an owner keeps them.  What it gets in f32 against
-autograd's bf16 of the same sums: off by that rounding, 2^-8 of the value."""
+"""``attention_block(norms=)``: its weights' gradients where an owner keeps them, and its backward in every form of the attention's.
+
+Tolerances: whole errors as in tests/test_qk_norm.py (the attention kernels' roundings of 2^-8 along the way, two to an output and four
+to a gradient); what an owner gets in f32 against autograd's bf16 of the same sums: its rounding, 2^-8 of the value."""
 import pytest
 import torch
 
 from mxllm import ops
+from mxllm.ops import attention
 
-from .test_qk_norm import EPS, HALF, _inputs
+from .test_qk_norm import EPS, HALF, _exact, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +63,31 @@ def test_owned_weights(gpu, block, fresh, who):
         assert p.grad is None and not p._mx_grad_fresh
         assert bool(((p._mx_grad32 - base - w).abs() <= HALF * size + 2.0 ** -20).all())
         assert len(told) == 1 and torch.equal(told[0], p._mx_grad32)
+
+
+@pytest.mark.parametrize("mode,budget", [(1, None), (2, None), (3, None), (3, 0)])
+@pytest.mark.parametrize("D,Hq,Hkv,S", [(32, 8, 2, 600), (64, 8, 2, 700), (128, 8, 1, 513), (128, 16, 2, 1030)])
+def test_longer_rows_in_every_form_of_the_backward(gpu, monkeypatch, D, Hq, Hkv, S, mode, budget):
+    """Sums of dQ by atomics, by ordered parts, by an image of dS, and that in chunks of heads; several partials of a key head."""
+    monkeypatch.setenv("MXLLM_ATTN_DQ_MODE", str(mode))
+    if budget is not None:
+        monkeypatch.setattr(attention, "_DS_BUDGET", budget)
+    dims = (2, S, Hq, Hkv, D)
+    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, *dims, seed=S)
+    do = torch.randn(2 * S, Hq * D, device=gpu, generator=torch.Generator(gpu).manual_seed(2)).bfloat16()
+    leaves = [t.clone().requires_grad_() for t in (qkv, wq, wk)]
+    out = ops.attention_block(leaves[0], cos, sin, *dims, norms=(*leaves[1:], EPS))
+    got = torch.autograd.grad(out, leaves, do)
+    exact = [t.double().cpu().requires_grad_() for t in (qkv, wq, wk)]
+    (q, k, v), _ = _exact(*exact, cos.cpu(), sin.cpu(), *dims)
+    k, v = (t.repeat_interleave(Hq // Hkv, 1) for t in (k, v))
+    s = (q @ k.transpose(2, 3)) * D ** -0.5
+    s = s.masked_fill(torch.ones(S, S).triu(1).bool(), float("-inf"))
+    want = (torch.softmax(s, -1) @ v).transpose(1, 2).reshape(2 * S, -1)
+    grads = torch.autograd.grad(want, exact, do.double().cpu())
+
+    def rel(a, b):
+        return float((a.detach().double().cpu() - b.detach()).norm() / b.detach().norm())
+
+    assert rel(out, want) < 2 * HALF
+    assert all(rel(a, b) < 4 * HALF for a, b in zip(got, grads)), [rel(a, b) for a, b in zip(got, grads)]
