@@ -208,15 +208,30 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
                  B: int, S: int, Hq: int, Hkv: int, D: int, eps: float = 1e-5, positions: torch.Tensor | None = None):
     """RMS norm of every query and key head (weights ``q_norm``, ``k_norm`` [D]) and its rotation, in one pass:
     qkv [B * S, (Hq + 2 Hkv) D] -> q [B, Hq, S, D], k and v [B, Hkv, S, D] as the attention kernels take them.
-    A row's position is its place in its sequence, or ``positions`` [B * S] int32 (packed documents); what lies outside
-    the table ``cos``, ``sin`` [positions, D / 2] comes out as NaN.  Differentiable once, in qkv and both weights
+    A row's position is its place in its sequence, for which the table ``cos``, ``sin`` [positions, D / 2] has to be long enough, or
+    ``positions`` [B * S] int32 (packed documents), where rows outside the table come out as NaN.  Differentiable once, in qkv and both weights
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
         if (q_norm.requires_grad or k_norm.requires_grad) and (_owned(q_norm) or _owned(k_norm)):
             _check_capture(qkv, q_norm, k_norm)
             return _QKNormRopeFn.apply(rows16(qkv), q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
         return native().qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+    _check_norm(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, positions)
     return ref.qk_norm_rope(qkv, q_norm, k_norm, cos, sin, B, S, Hq, Hkv, D, eps, positions)
+
+
+def _check_norm(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, positions=None) -> None:
+    """What the kernel's binding refuses of the operands' shapes, for the plain form."""
+    if Hkv < 1 or Hq < Hkv or Hq % Hkv:
+        raise ValueError(f"query heads in whole groups of a key head, got {Hq} of {Hkv}")
+    if qkv.dim() != 2 or tuple(qkv.shape) != (B * S, (Hq + 2 * Hkv) * D):
+        raise ValueError(f"qkv [B S, (Hq + 2 Hkv) D] = [{B * S}, {(Hq + 2 * Hkv) * D}], got {list(qkv.shape)}")
+    if any(tuple(w.shape) != (D,) for w in (wq, wk)):
+        raise ValueError(f"q_norm, k_norm: [{D}]")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2 or cos.shape[0] < (S if positions is None else 1):
+        raise ValueError(f"cos, sin: [positions, D / 2], rows up to {S}, got {list(cos.shape)}, {list(sin.shape)}")
+    if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (B * S,)):
+        raise ValueError(f"positions: int32 [{B * S}], got {positions.dtype} {list(positions.shape)}")
 
 
 def attention_block(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, B: int, S: int, Hq: int,
@@ -231,6 +246,7 @@ def attention_block(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, B: 
         if use_native(qkv):
             _check_capture(qkv, wq, wk)
             return _NormAttnBlockFn.apply(rows16(qkv), wq, wk, cos, sin, B, S, Hq, Hkv, D, eps, causal, out_pad, grad_pad)
+        _check_norm(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D)
         q, k, v = ref.qk_norm_rope(qkv, wq, wk, cos, sin, B, S, Hq, Hkv, D, eps)
         return ref.attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal=causal).reshape(B * S, Hq * D)
     if use_native(qkv):

@@ -162,7 +162,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: li
 
 
 def read(pages: Pages, slots: torch.Tensor | None, starts: torch.Tensor, ends: torch.Tensor, n: int):
-    """(k, v) bf16 [B, Hkv, n, D] of positions starts[b] + i, i < n, of slot slots[b] (int32 [B]); zero from ends[b] on.
+    """(k, v) bf16 [B, Hkv, n, D] of positions starts[b] + i, i < n, of slot slots[b] (int32 [B]; None: the rows' numbers); zero from
+    ends[b] on, ahead of position 0, behind the block table and of a slot that is none.
     Exact: bf16 holds every value of the cache (under exponent bytes of 3 and more)."""
     if use_native(pages.k):
         return native().kv8_read(*pages, slots, starts, ends, n)
@@ -224,7 +225,7 @@ def _check_pages(pages: Pages) -> None:
     if (any(t.dtype != torch.uint8 for t in (k, v, ke, ve)) or k.dim() != 4 or v.shape != k.shape or k.shape[2] % GROUP
             or 0 in k.shape or tuple(ke.shape) != want or tuple(ve.shape) != want):
         raise ValueError("8-bit cache: uint8 codes [pages, Hkv, block, D] (block a multiple of 16), exponents [pages, Hkv, block / 16]")
-    if table.dtype != torch.int32 or table.dim() != 2:
+    if table.dtype != torch.int32 or table.dim() != 2 or 0 in table.shape:
         raise ValueError("block table: int32 [slots, max_pages]")
 
 
@@ -235,7 +236,7 @@ def _check_rows(qkv, cos, sin, pages: Pages, Hq: int, q_norm, k_norm) -> tuple[i
         raise ValueError(f"query heads in whole groups of a key head, got {Hq} of {Hkv}")
     if qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"qkv [T, (Hq + 2 Hkv) D] = [.., {(Hq + 2 * Hkv) * D}], got {list(qkv.shape)}")
-    if cos.shape[-1] != D // 2 or cos.shape != sin.shape:
+    if cos.dim() != 2 or cos.shape[0] == 0 or cos.shape[1] != D // 2 or cos.shape != sin.shape:
         raise ValueError("cos, sin: [positions, D / 2]")
     if (q_norm is None) != (k_norm is None) or any(w is not None and tuple(w.shape) != (D,) for w in (q_norm, k_norm)):
         raise ValueError("weights [D] of both norms, or of none")
