@@ -14,8 +14,8 @@
 //
 // Bound by memory (prompts) and by a few dependent loads (single tokens).  A wave has one group of one head: 16 rows of four
 // lanes, each with D / 8 pairs (i, i + D / 2), so the rotation needs no neighbour, a norm two lane swaps, and the group's
-// largest value one fold of the wave.  4,096 rows of 48 heads of 128 behind 1,003 positions, normed: 26 us (109 MB, 4.1 TB/s; a large
-// copy runs at 4.9), read back 6.4 (25 MB).  64 single tokens of 80 heads of 128 6.6 us, one of 48 heads of 64 3.9.
+// largest value one fold of the wave.  4,096 rows of 48 heads of 128 behind 1,003 positions, normed: 26.5 us (109 MB, 4.1 TB/s; a copy
+// of as much runs at 5.9), read back 6.4 (25 MB).  64 single tokens of 80 heads of 128 6.6 us, one of 48 heads of 64 3.9.
 #include "kv8.h"
 
 namespace mx {

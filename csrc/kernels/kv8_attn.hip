@@ -2,7 +2,7 @@
 //   o = softmax(q k^T scale) v over positions 0 .. pos, queries of a group of heads sharing a key/value head.
 //
 // Bound by memory: a key and a value of a head are 2 D bytes, half of a bf16 cache's, each read once for all query heads of the
-// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 48 us, of which the merge 4; a linear read of as much takes 45.
+// group.  8 sequences of 16,384 keys (8 heads of 128, 269 MB) 48 us, of which the merge 4.5; a linear read of as much takes 39.
 //
 //   S^T[key][head] = 2^(ek - 127) scale log2(e) (K . Q^T),  O^T[d][head] += (2^(ev - 127) V^T) . P
 // by v_mfma_f32_16x16x32_bf16 on codes that become bf16 in registers, where they are exact, the units' (16 positions) powers of
@@ -16,13 +16,14 @@
 // are not kept in the caches, the next tile's while this one is worked on, and nothing waits for another wave.  A lane (c, g)
 // then takes row c of each unit, pieces of 16 bytes 64 h + 16 g (a dot product does not mind the order of channels, and queries
 // are laid out alike), and of eight value rows its D / 16 channels, whose bytes are put together row by row as the product
-// reads them.  Us with what was there before, memory's caches cold / as three calls in turn leave them:
+// reads them.  Us with what was there before (a weight was one number then, parts lay by row), memory's caches cold / as three calls
+// in turn leave them:
 //   a lane's rows straight to registers, kept in the caches    32 x 100 .. 2000 of 128 19.6 / 16.6, 8 x 16384 54.9 / 54.6
 //   the same, not kept (rows of half a line: 40 x 1000 .. 4000 of 64 18.2 -> 19.7)      20.6 / 20.0,            49.8 / 49.3
 //   whole rows by LDS, not kept                                                        18.2 / 17.4,            49.8 / 48.9
 //   and the next tile on its way                                                       16.1 / 15.4,            47.8 / 47.3
-// and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 66.7 cold, 6.1 TB/s; one of 700 keys does not mind.  (Keys of the tile after
-// next asked for as soon as a tile's are read, values alike, was 2 to 8 % slower.)
+// and 64 x 2048 .. 4096 78.3 -> 71.9 -> 69.1 -> 66.7 cold (now 70, 5.9 TB/s; a linear read of as much 59); one of 700 keys does not
+// mind.  (Keys of the tile after next asked for as soon as a tile's are read, values alike, was 2 to 8 % slower.)
 //
 // Rows are whole (a workgroup each, nothing to merge) or cut: the units of all sequences in a row are dealt in equal
 // shares, one a workgroup of a KV head, whose waves share what it has of a sequence, and sequences that were cut are merged by a
@@ -287,9 +288,9 @@ __device__ __forceinline__ int kv8_len(int pos, int slot, const Kv8Pages& pg, in
 __device__ __forceinline__ int kv8_units(int len) { return (len + kUnit - 1) / kUnit; }
 // Units that a row is dealt as: its own and `pad` for what a workgroup spends on a row beside its keys (48 KB of them), none where no
 // workgroup has parts of two rows (B up to 64: a lane has a row's units), so that shares that are whole turns of the waves stay
-// so.  Us with 6 always, with 6 / 12 / 24 / 48 where rows meet: 1 row (8 heads of 128) of 4,096 keys 10.2, 9.5 all; 2 of 4,096 11.2, 10.4; 8 of
-// 16,384 49.7, 47.6;  4 of 20000 .. 30000 39.1, 39.4 / 39.7 / 40.1 / 40.2;  8 of 64 of 4000 .. 8192 17.8, 18.1 / 17.6 / 17.3 / 16.7;  32 of 2 heads of 32 of
-// 4096 .. 8192 13.1, 13.8 / 13.4 / 13.2 / 12.5.
+// so.  Us with 6 always, with 6 / 12 / 24 / 48 where rows meet: 1 sequence (8 heads of 128) of 4,096 keys 9.6, 8.8 all; 2 of 4,096 11.7,
+// 10.0; 8 of 16,384 48.5, 47.9;  4 of 20000 .. 30000 37.5, 38.3 / 37.8 / 38.4 / 38.0;  8 (heads of 64) of 4000 .. 8192 16.5, 17.3 / 17.1 / 16.9
+// / 16.6;  32 of 2 heads of 32 of 4096 .. 8192 13.5, 13.9 / 13.8 / 13.4 / 12.8.
 constexpr int kLeast = 8;
 constexpr int kv8_pads(int D) { return 48 * 32 / D; }
 __device__ __forceinline__ int kv8_dealt(int units, int pad) { return units ? units + pad : 0; }
@@ -549,26 +550,28 @@ __global__ void __launch_bounds__(C* G)
 
 using namespace mx;
 
-// Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB (a CU's 60 GB/s,
-// however many waves); cutting costs a merge and more ends, 2 to 7 us.  Rows that leave no CU alone are better off by four
-// waves, where a CU has the next row's workgroup beside this one's end.  Us, cold, with whole rows of 4 / 8 waves, and cut:
-//   heads of 128: 8 rows of 700 keys 7.5 / 7.2, 8.3; of 1,024 8.7 / 8.6, 8.3; of 2,048 13.4 / 13.2, 8.3;  32 of 1,500 11.4 / 11.5, 11.1;
-//     64 of 1000 .. 2000 13.7 / 13.9, 14.4; of 16,384 88.9 / 84.8, 47.8;  128 of 1000 .. 2000 14.6 / 15.1, 19.2; of 2000 .. 4096 24.8 / 25.6,
-//     26.1;  192 of 100 .. 4096 25.5 / 26.6, 27.2;  256 of 100 .. 2000 16.0 / 16.8, 21.3; of 100 .. 4096 27.4 / 28.4, 33.6;  512 of 30 .. 512
-//     10.6 / 12.8, 20.0; of 2048 .. 4096 66.8 / 70.1, 72.2
-//   of 64: 8 of 700 6.1 / 5.4, 7.5; of 2,048 11.3 / 8.9, 8.1;  64 of 1000 .. 3000 14.6 / 10.9, 12.4;  128 of 500 .. 2000 11.5 / 9.1, 13.9; of 1000
-//     .. 6000 29.2 / 19.6, 18.5;  192 of 100 .. 4000 20.0 / 14.8, 18.4;  320 of 1000 .. 8000 45.7 / 47.9, 39.6;  384 of 100 .. 2000 14.0 / 14.8,
-//     19.1;  512 of 2048 .. 4096 36.1 / 36.8, 42.5
-//   of 32: 64 of 4096 .. 8192 31.1 / 19.5, 13.2;  512 of 1000 .. 8000 39.5 / 35.9, 38.1;  1,024 of 30 .. 512 7.2 / 7.4, 18.8
+// Waves of a workgroup that takes a whole row, 0: rows are cut.  A row takes a workgroup 4.5 us for 256 KB of heads of 128 (a CU's
+// 60 GB/s, however many waves); cutting costs a merge and more ends, 2 to 11 us.  The bounds are in keys whatever D is: a workgroup's
+// time goes by its tiles of 32 as much as by their bytes (2,048 keys 14.5 us of 128, 10.7 of 64).  Rows that leave no CU alone are
+// better off by four waves or within 3 % of it, where a CU has the next row's workgroup beside this one's end.  Us, cold, of a call
+// in a graph (1.5 of it between launches), with whole rows of 4 / 8 waves, and cut:
+//   heads of 128: 8 rows of 700 keys 8.9 / 8.7, 9.8; of 1,024 10.4 / 9.7, 10.1; of 2,048 15.8 / 14.5, 10.3;  32 of 1,500 13.2 / 12.4, 12.1;
+//     64 of 1000 .. 2000 14.8 / 13.9, 16.0; of 16,384 96.1 / 87.3, 50.4;  128 of 1000 .. 2000 15.7 / 15.3, 21.3; of 2000 .. 4096 25.9 / 25.4,
+//     27.8;  192 of 100 .. 4096 27.7 / 27.7, 29.2;  256 of 100 .. 2000 17.6 / 17.7, 22.3; of 100 .. 4096 31.2 / 31.6, 34.3;  512 of 30 .. 512
+//     11.8 / 14.5, 21.5; of 2048 .. 4096 70.1 / 69.8, 71.6
+//   of 64: 8 of 700 7.7 / 6.9, 9.2; of 2,048 13.0 / 10.7, 9.3;  64 of 1000 .. 3000 16.3 / 13.0, 13.3 (cut, its bound being 2,048);  128 of 500 ..
+//     2000 12.8 / 10.7, 15.5; of 1000 .. 6000 31.0 / 22.7, 20.2;  192 of 100 .. 4000 21.6 / 17.1, 20.3;  320 of 1000 .. 8000 48.6 / 49.1, 39.0;
+//     384 of 100 .. 2000 16.0 / 16.0, 21.5;  512 of 2048 .. 4096 38.0 / 38.9, 42.1
+//   of 32: 64 of 4096 .. 8192 33.9 / 22.8, 14.4;  512 of 1000 .. 8000 41.6 / 36.9, 39.4 (cut);  1,024 of 30 .. 512 8.9 / 9.4, 22.2
 // Rows of few keys beside a long one are what whole rows are worst at: the bounds keep that within some 12 us.
 static int kv8_waves(int64_t rows, int64_t cap, int D) {
   if (cap > (rows >= 128 ? 4096 : rows >= 32 ? 32 * rows : 1024)) return 0;
   return rows >= (D == 128 ? 128 : D == 64 ? 384 : 1024) ? 4 : 8;
 }
 // Workgroups of a KV head where keys are dealt evenly: one a CU of 256, of four waves with heads of 128, of eight with smaller ones.
-// Us with 512 of four waves, 256 of eight, 256 of four: 8 rows (8 heads) of 128 of 4,096 keys 10.8, 10.4, 10.2, of 32,768 20.2, 18.8, 18.6;
-// 64 of 16,384 49.3, 50.1, 49.7; 512 of 500 .. 8192 94.6, 96.4, 93.3;  8 of 64 of 16,384 12.5, 11.0, 11.0; 64 of 4000 .. 8192 17.6, 17.7,
-// 18.1;  64 of 32 of 4096 .. 8192 13.7, 13.1, 14.4.  (768 of four waves 23.8 and 55.0 where 512 have 20.2 and 49.3.)
+// Us with 512 of four waves, 256 of eight, 256 of four: 8 rows (a sequence of 8 heads) of 128 of 4,096 keys 9.8, 8.9, 8.9, of 32,768 19.0,
+// 17.7, 17.4; 64 of 16,384 48.0, 48.7, 47.9; 512 of 500 .. 8192 97.9, 99.2, 95.2;  8 of 64 of 16,384 11.4, 10.3, 10.3; 64 of 4000 .. 8192 15.6,
+// 16.5, 16.4;  64 of 32 of 4096 .. 8192 12.7, 12.7, 14.3.  (768 of four waves 23.8 and 54.5 where 512 have 19.0 and 48.0.)
 static int kv8_shares(int Hkv) { return Hkv < 256 ? (256 + Hkv - 1) / Hkv : 1; }
 
 // places for parts that a query head has (of part_ml [Hq, places, 2], part_o [Hq, places, D]); 0: rows are whole
@@ -609,7 +612,8 @@ void launch(const Launch& a) {
       a.pos, a.slots, a.pg.table, a.q, a.pg.k, a.pg.v, a.pg.ke, a.pg.ve, a.pg.slots, a.pg.maxp, a.pg.block, a.pg.pages, Hkv,
       a.part_ml, a.part_o, a.out, a.B, a.Hq, a.cap, a.sl);
   const int rows = a.B * a.Hq;
-  if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 17.5 -> 10.8 us, 1 x 32768 34.1 -> 20.3
+  if (rows <= 512)  // few rows are waited for part by part: 1 x 4096 keys 15.2 -> 8.8 us, 1 x 32768 23.8 -> 17.5 (8 x 16384, of four parts a
+                    // row, 47.1 -> 48.1; 64 x 500 .. 8192, 4,096 rows, would be 95 -> 107)
     kv8_merge_kernel<D, 32, 8><<<rows * (D / 32), 256, 0, a.stream>>>(a.part_ml, a.part_o, a.pg, a.pos, a.slots, a.out, a.B,
                                                                       a.Hq, W, a.cap);
   else

@@ -209,7 +209,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     """RMS norm of every query and key head (weights ``q_norm``, ``k_norm`` [D]) and its rotation, in one pass:
     qkv [B * S, (Hq + 2 Hkv) D] -> q [B, Hq, S, D], k and v [B, Hkv, S, D] as the attention kernels take them.
     A row's position is its place in its sequence, for which the table ``cos``, ``sin`` [positions, D / 2] has to be long enough, or
-    ``positions`` [B * S] int32 (packed documents), where rows outside the table come out as NaN.  Differentiable once, in qkv and both weights
+    ``positions`` [B * S] int32 (packed documents), where rows outside the table come out as NaN.  Differentiable once, in qkv and both weights, not under ``torch.func``
     (csrc/kernels/qk_norm.hip)."""
     if use_native(qkv):
         if (q_norm.requires_grad or k_norm.requires_grad) and (_owned(q_norm) or _owned(k_norm)):

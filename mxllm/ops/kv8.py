@@ -164,7 +164,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: li
 def read(pages: Pages, slots: torch.Tensor | None, starts: torch.Tensor, ends: torch.Tensor, n: int):
     """(k, v) bf16 [B, Hkv, n, D] of positions starts[b] + i, i < n, of slot slots[b] (int32 [B]; None: the rows' numbers); zero from
     ends[b] on, ahead of position 0, behind the block table and of a slot that is none.
-    Exact: bf16 holds every value of the cache (under exponent bytes of 3 and more)."""
+    Exact: bf16 holds every value of the cache (under exponent bytes of 3 and more, up to the end of f32)."""
     if use_native(pages.k):
         return native().kv8_read(*pages, slots, starts, ends, n)
     B = starts.shape[0]
