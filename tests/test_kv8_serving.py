@@ -37,7 +37,7 @@ def _worker(rank, world, port, out_q):
     everyone = [torch.zeros_like(logits) for _ in range(world)]
     dist.all_gather(everyone, logits)
     if rank == 0:
-        out_q.put((logits, all(torch.equal(logits, x) for x in everyone), tuple(engine.kv.k_exp[0].shape)))
+        out_q.put((logits.numpy(), all(torch.equal(logits, x) for x in everyone), tuple(engine.kv.k_exp[0].shape)))
     runtime.cleanup()
 
 
@@ -53,6 +53,7 @@ def test_tensor_parallel_shards_keep_their_heads(world):
     for p in procs:
         p.start()
     got, same, exps = q.get(timeout=240)
+    got = torch.from_numpy(got)  # (a tensor would be shared, and its process is gone)
     for p in procs:
         p.join(60)
         assert p.exitcode == 0
