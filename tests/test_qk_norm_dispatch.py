@@ -96,3 +96,25 @@ def test_rows_at_odd_places_have_gradients(gpu):
         assert not back[:, :shift].any() and not back[:, shift + qkv.shape[1]:].any()
         got.append([*out, back[:, shift:shift + qkv.shape[1]]])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_attention_block_with_norms(gpu):
+    """The block's own autograd: a trace has its ops, and many backwards at once are those one by one."""
+    (qkv, wq, wk, *_), cos, sin = _inputs(gpu, *DIMS)
+
+    def run(x, a, b):
+        return ops.attention_block(x, cos, sin, *DIMS, norms=(a, b, EPS))
+
+    traced = make_fx(run, tracing_mode="real")(qkv, wq, wk)
+    names = [n.target._schema.name for n in traced.graph.nodes if isinstance(n.target, torch._ops.OpOverload)]
+    assert names.count(FORWARD) == 1
+    other, _, _ = _inputs(gpu, *DIMS, seed=5)
+    for given in ((qkv, wq, wk), other[:3]):
+        assert torch.equal(traced(*given), run(*given))
+    leaves = [t.clone().requires_grad_() for t in (qkv, wq, wk)]
+    out = run(*leaves)
+    do = torch.randn(2, *out.shape, device=gpu, generator=torch.Generator(gpu).manual_seed(1)).bfloat16()
+    got = torch.autograd.grad(out, leaves, do, is_grads_batched=True, retain_graph=True)
+    for i in range(2):
+        want = torch.autograd.grad(out, leaves, do[i], retain_graph=True)
+        assert all(torch.equal(x[i], y) for x, y in zip(got, want))
